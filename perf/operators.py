@@ -283,12 +283,12 @@ def _run_plain(s):
         out["dx"] = torch.cat([d[a:b] @ w[e].t() for e, (a, b) in enumerate(spans)]).to(dt)
         out["dw"] = torch.stack([x[a:b].t() @ d[a:b] for a, b in spans]).to(dt)
         if case["bias"]:
-            out["db"] = torch.stack([d[a:b].sum(0) for a, b in spans])
+            out["db"] = torch.stack([d[a:b].sum(0) for a, b in spans]).to(dt)
     else:
         out["dx"] = (d @ w).to(dt)
         out["dw"] = (d.t() @ x).to(dt)
         if case["bias"]:
-            out["db"] = d.sum(0)
+            out["db"] = d.sum(0).to(dt)
     return out
 
 
@@ -317,7 +317,7 @@ def work(case):
     if not case["train"]:
         return dict(bytes=int(fwd), flops=2 * m * I * O)
     # backward, each input of the pass read once: dy in; pre, dx, dw, db out
-    bwd = es * (m * yc + m * O + m * I + groups * I * O) + (4 * groups * O if case["bias"] else 0)
+    bwd = es * (m * yc + m * O + m * I + groups * I * O) + (es * groups * O if case["bias"] else 0)
     return dict(bytes=int(fwd + bwd), flops=6 * m * I * O)
 
 
