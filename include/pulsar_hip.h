@@ -36,6 +36,16 @@ extern "C" {
 #define PULSAR_F32 0
 #define PULSAR_BF16 1
 
+/* Activations of the linear ops' epilogue. SwiGLU halves the columns: silu(first half) times
+ * the second. GELU is the erf form, GELU_TANH its tanh approximation. */
+#define PULSAR_ACT_NONE 0
+#define PULSAR_ACT_RELU 1
+#define PULSAR_ACT_SILU 2
+#define PULSAR_ACT_GELU 3
+#define PULSAR_ACT_GELU_TANH 4
+#define PULSAR_ACT_SIGMOID 5
+#define PULSAR_ACT_SWIGLU 6
+
 /* Thread-local message of the last failing call on this thread. */
 const char* pulsar_last_error(void);
 /* ABI version of this header (bumped on any signature change). */
@@ -216,6 +226,74 @@ int pulsar_causal_conv1d_k4_backward(const void* dout, const void* x, const floa
                                      float* dw, int64_t B, int64_t T, int64_t D, int dtype,
                                      hipStream_t stream);
 
+
+/* ---------------------------------------------------------------------------------
+ * Products with their epilogues: the dense ones of the shared expert and the projections,
+ * the ragged ones of the routed experts over every assignment (no capacity, nothing
+ * dropped). No reference binding: the reference calls torch's linear and bmm for these
+ * (src/model.py:923-949, :1432-1483).
+ *   bf16 and fp32; fp32 sums; pre-activation values, bias, activation and residual are taken
+ *   in fp32 and each output is rounded once. The gradients take act'(pre) dy rounded to the
+ *   activation dtype into their products. Same inputs give the same bits on every call.
+ *   1 <= d_in, d_out, 1 <= groups <= 65536, rows < 2^31 - 256.
+ * ------------------------------------------------------------------------------- */
+
+/* moe_group_rows(topk_idx, E): the assignments [N, K] sorted by expert, stable.
+ *   offsets int32 [E+1]: expert e's rows are [offsets[e], offsets[e+1]);
+ *   rows int32 [N K]: the token of each row, -1 past offsets[E];
+ *   slots int32 [N, K]: the row of each assignment, -1 for ids outside [0, E) (padding), which
+ *   take no row. E <= 1024. workspace: the given number of bytes (-1: bad shape) of device
+ *   memory, 4-byte aligned, any contents; none when it is 0. */
+int64_t pulsar_moe_group_rows_workspace_bytes(int64_t N, int64_t K, int64_t E);
+int pulsar_moe_group_rows(const int64_t* topk_idx, int32_t* offsets, int32_t* rows, int32_t* slots,
+                          int64_t N, int64_t K, int64_t E, void* workspace, hipStream_t stream);
+
+/* y = act(x w^T + bias) + residual.
+ *   x: [rows, d_in], row stride x_rs; w element (o, i) at o w_out + i w_in, one of the strides 1;
+ *   bias: [d_out] of bias_dtype, nullable; residual: [rows, columns of y], row stride
+ *   residual_rs, nullable; y: contiguous [rows, d_out] (SwiGLU: d_out / 2); pre: contiguous
+ *   [rows, d_out], the values the activation took, for the backward call, nullable. */
+int pulsar_fused_linear_forward(const void* x, int64_t x_rs, const void* w, int64_t w_out,
+                                int64_t w_in, const void* bias, int bias_dtype,
+                                const void* residual, int64_t residual_rs, void* y, void* pre,
+                                int64_t rows, int64_t d_in, int64_t d_out, int activation,
+                                int dtype, hipStream_t stream);
+
+/* Its gradients: dx contiguous [rows, d_in]; dw contiguous in w's own order (w_in == 1:
+ * [d_out][d_in], else [d_in][d_out]); db [d_out] in dtype, nullable (not computed). dy
+ * contiguous; the residual's gradient is dy. pre: the forward's (unused without activation).
+ * workspace: the given number of bytes of device memory, 16-byte aligned, any contents. */
+int64_t pulsar_fused_linear_backward_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out,
+                                                     int activation, int dtype);
+int pulsar_fused_linear_backward(const void* dy, const void* x, int64_t x_rs, const void* w,
+                                 int64_t w_out, int64_t w_in, const void* pre, void* dx, void* dw,
+                                 void* db, int64_t rows, int64_t d_in, int64_t d_out,
+                                 int activation, int dtype, void* workspace, hipStream_t stream);
+
+/* y[i] = act(x[row_index[i]] w[e] + bias[e]) for the rows i of group e, [offsets[e], offsets[e+1]).
+ *   x: [x_rows, d_in], row stride x_rs; row_index int32 [rows], nullable (row i itself; x_rows
+ *   == rows); an index outside x reads as a row of zeros. offsets int32 [groups + 1], rising
+ *   from 0 to at most rows; rows past offsets[groups] become zeros in y and pre. w element
+ *   (e, i, o) at e w_group + i w_in + o w_out, one of w_in and w_out 1; bias [groups, d_out]. */
+int pulsar_grouped_linear_forward(const void* x, int64_t x_rs, int64_t x_rows,
+                                  const int32_t* row_index, const int32_t* offsets, const void* w,
+                                  int64_t w_group, int64_t w_in, int64_t w_out, const void* bias,
+                                  int bias_dtype, void* y, void* pre, int64_t rows,
+                                  int64_t groups, int64_t d_in, int64_t d_out, int activation,
+                                  int dtype, hipStream_t stream);
+
+/* Its gradients: dx contiguous [rows, d_in], a row for each row of y (the sum over the rows that
+ * share a row of x is the caller's: pulsar_moe_dispatch_backward), zeros past offsets[groups];
+ * dw contiguous in w's own order, groups outermost, zeros for empty groups; db [groups, d_out]
+ * in dtype, nullable. */
+int64_t pulsar_grouped_linear_backward_workspace_bytes(int64_t rows, int64_t groups, int64_t d_in,
+                                                       int64_t d_out, int activation, int dtype);
+int pulsar_grouped_linear_backward(const void* dy, const void* x, int64_t x_rs, int64_t x_rows,
+                                   const int32_t* row_index, const int32_t* offsets, const void* w,
+                                   int64_t w_group, int64_t w_in, int64_t w_out, const void* pre,
+                                   void* dx, void* dw, void* db, int64_t rows, int64_t groups,
+                                   int64_t d_in, int64_t d_out, int activation, int dtype,
+                                   void* workspace, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------------
  * Decode engine: prefill + self-speculative decode of a batch of sequences.

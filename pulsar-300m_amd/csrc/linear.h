@@ -1,0 +1,90 @@
+// Dense and ragged products with their epilogues (linear.hip): arguments and the parts shared
+// with the activation kernels.
+#pragma once
+
+#include "common.h"
+
+namespace pulsar {
+
+typedef __bf16 lin_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float lin_f32x4 __attribute__((ext_vector_type(4)));
+
+// One launch: C[m][n] = sum_k A[m][k] B[n][k] over each group.
+//   Products (forward, gradient of x): m runs over the ragged rows, n and k over the weight's
+//   two dimensions. Rows of group e are [offsets[e], offsets[e + 1]); rows past the last group
+//   are written as zeros. offsets == nullptr: one group of `rows` rows.
+//   Weight gradient: m and n run over the weight's dimensions, k over the rows of the group.
+struct LinearArgs {
+  const void* A;
+  const void* B;
+  int64_t lda, ldb;        // elements from one row of the stored matrix to the next
+  int64_t b_group;         // products: elements from one group's weight to the next
+  const int32_t* a_rows;   // row i of A is stored row a_rows[i] (nullptr: i)
+  const int32_t* b_rows;   // the same of B (weight gradient)
+  int64_t a_nrows, b_nrows;  // stored rows; an index outside them reads as a row of zeros
+  const int32_t* offsets;
+  int groups;
+  int rows;                // ragged rows in all
+  int M, N, K;             // M: weight gradient only; K: products only
+  void* C;
+  int64_t ldc, c_group;
+  void* pre;               // products: pre-activation values (nullptr: not kept)
+  int64_t ldpre;
+  const void* bias;        // products: [groups][N] (nullptr: none)
+  int bias_dtype;
+  const void* residual;    // products: added after the activation (nullptr: none)
+  int64_t ldr;
+  int act;
+  void* db;                // weight gradient: [groups][dim] sums of dpre's rows, storage type
+  float* part;             // weight gradient in splits: [split][groups][M][N] partial sums
+  float* part_db;          //   and [split][groups][dim]
+  int splits;
+  int tiles_m, tiles_n;    // weight gradient: tiles of one group
+  int max_tiles;           // products: bound of the row tiles
+};
+
+// The activation of v, and its derivative. expf / erff / tanhf: the fp32 kernels' outputs are
+// held to fp32 rounding.
+__device__ __forceinline__ float act_value(int act, float v) {
+  switch (act) {
+    case PULSAR_ACT_RELU: return v < 0.f ? 0.f : v;  // NaN stays NaN
+    case PULSAR_ACT_SILU: return v * sigmoidf_(v);
+    case PULSAR_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678f));
+    case PULSAR_ACT_GELU_TANH: {
+      // 0.5 (1 + tanh(u)) = sigmoid(2 u)
+      const float u = 0.79788456f * (v + 0.044715f * v * v * v);
+      return v * sigmoidf_(2.f * u);
+    }
+    case PULSAR_ACT_SIGMOID: return sigmoidf_(v);
+    default: return v;
+  }
+}
+// The slopes are taken at v held to a range past which they are 0 or 1 in fp32, so that no
+// infinite v meets a zero factor (NaN passes through).
+__device__ __forceinline__ float hold(float v, float b) { return v > b ? b : (v < -b ? -b : v); }
+__device__ __forceinline__ float act_slope(int act, float v) {
+  switch (act) {
+    case PULSAR_ACT_RELU: return v > 0.f ? 1.f : (v <= 0.f ? 0.f : v);
+    case PULSAR_ACT_SILU: {
+      v = hold(v, 100.f);
+      const float s = sigmoidf_(v);
+      return s * (1.f + v * (1.f - s));
+    }
+    case PULSAR_ACT_GELU:
+      v = hold(v, 30.f);
+      return 0.5f * (1.f + erff(v * 0.70710678f)) + v * 0.39894228f * expf(-0.5f * v * v);
+    case PULSAR_ACT_GELU_TANH: {
+      v = hold(v, 30.f);
+      const float v2 = v * v;
+      const float s = sigmoidf_(1.59576912f * v * (1.f + 0.044715f * v2));
+      return s + v * s * (1.f - s) * 1.59576912f * (1.f + 0.134145f * v2);
+    }
+    case PULSAR_ACT_SIGMOID: {
+      const float s = sigmoidf_(v);
+      return s * (1.f - s);
+    }
+    default: return 1.f;
+  }
+}
+
+}  // namespace pulsar

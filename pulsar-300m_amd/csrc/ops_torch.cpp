@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -314,6 +315,145 @@ PyObject* moe_combine_backward(const Args& a) {
   return pair(de, dw, true);
 }
 
+// Row stride of a tensor read as [rows, last dimension]: 2-dimensional with any row stride, or
+// contiguous.
+int64_t row_stride(const Tensor& t, const char* name) {
+  const int64_t n = t.size(-1), rows = n ? t.numel() / n : 0;
+  if (rows <= 1) {
+    TORCH_CHECK(n <= 1 || t.stride(-1) == 1, name, " must have stride(-1) == 1");
+    return n;
+  }
+  if (t.is_contiguous()) return n;
+  TORCH_CHECK(t.dim() == 2 && (n == 1 || t.stride(1) == 1), name,
+              " must be contiguous, or 2-dimensional with stride(-1) == 1");
+  return t.stride(0);
+}
+// Strides of a weight's last two dimensions, one of them 1 (a dimension of size 1 has no stride
+// of its own).
+void weight_strides(const Tensor& w, int64_t& s0, int64_t& s1) {
+  const int64_t n0 = w.size(-2), n1 = w.size(-1);
+  s0 = w.stride(-2);
+  s1 = w.stride(-1);
+  if (n1 == 1) s1 = 1;
+  if (n0 == 1) s0 = s1 == 1 ? n1 : 1;
+  TORCH_CHECK(s0 == 1 || s1 == 1, "weight must have a unit stride in one of its last two dimensions");
+}
+// A gradient of weight w, dense in w's own order of the last two dimensions.
+Tensor weight_grad(const Tensor& w, bool last_contiguous) {
+  std::vector<int64_t> shape = w.sizes().vec();
+  if (last_contiguous) return make(w, shape);
+  std::swap(shape[shape.size() - 1], shape[shape.size() - 2]);
+  return make(w, shape).transpose(-2, -1);
+}
+PyObject* triple(const Tensor& a, const Tensor& b, const Tensor& c, bool list) {
+  PyObject* o[3] = {out(a), out(b), c.defined() ? out(c) : Py_NewRef(Py_None)};
+  PyObject* r = o[0] && o[1] && o[2] ? (list ? PyList_New(3) : PyTuple_New(3)) : nullptr;
+  if (!r) {
+    for (PyObject* x : o) Py_XDECREF(x);
+    throw python_error();
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (list)
+      PyList_SET_ITEM(r, i, o[i]);
+    else
+      PyTuple_SET_ITEM(r, i, o[i]);
+  }
+  return r;
+}
+
+// (topk_idx, E) -> (offsets, rows, slots)
+PyObject* moe_group_rows(const Args& a) {
+  const Tensor& idx = a.t(0);
+  const int64_t N = idx.size(0), K = idx.size(1), E = a.i64(1);
+  const c10::DeviceGuard guard(idx.device());
+  const int64_t bytes = pulsar_moe_group_rows_workspace_bytes(N, K, E);
+  Tensor o = make(idx, {E + 1}, at::kInt), r = make(idx, {N * K}, at::kInt);
+  Tensor s = make(idx, {N, K}, at::kInt), ws;
+  if (bytes > 0) ws = make(idx, {bytes / 4}, at::kInt);
+  run(pulsar_moe_group_rows, p<int64_t>(idx), q<int32_t>(o), q<int32_t>(r), q<int32_t>(s), N, K, E,
+      const_cast<void*>(p(ws)), stream(idx));
+  return triple(o, r, s, false);
+}
+
+// (x, weight [O, I], bias, residual, activation, save_pre) -> y or (y, pre)
+PyObject* fused_linear_forward(const Args& a) {
+  const Tensor &x = a.t(0), &w = a.t(1);
+  const Tensor b = a.opt(2), res = a.opt(3);
+  const int64_t act = a.i64(4), I = x.size(-1), O = w.size(0), rows = x.numel() / I;
+  int64_t so, si;
+  weight_strides(w, so, si);
+  const int64_t xs = row_stride(x, "x"), rs = res.defined() ? row_stride(res, "residual") : 0;
+  const c10::DeviceGuard guard(x.device());
+  std::vector<int64_t> shape = x.sizes().vec();
+  Tensor pre;
+  shape.back() = O;
+  if (a.i64(5)) pre = make(x, shape);
+  if (act == PULSAR_ACT_SWIGLU) shape.back() = O / 2;
+  Tensor y = make(x, shape);
+  run(pulsar_fused_linear_forward, p(x), xs, p(w), so, si, p(b), b.defined() ? code(b) : 0, p(res),
+      rs, q(y), pre.defined() ? q(pre) : nullptr, rows, I, O, (int)act, code(x), stream(x));
+  return pre.defined() ? pair(y, pre, false) : out(y);
+}
+
+// (dy, x, weight [O, I], pre, activation, bias) -> [dx, dw, db]
+PyObject* fused_linear_backward(const Args& a) {
+  const Tensor &dy = a.t(0), &x = a.t(1), &w = a.t(2);
+  const Tensor pre = a.opt(3);
+  const int64_t act = a.i64(4), I = x.size(-1), O = w.size(0), rows = x.numel() / I;
+  int64_t so, si;
+  weight_strides(w, so, si);
+  const int64_t xs = row_stride(x, "x");
+  const c10::DeviceGuard guard(x.device());
+  Tensor dx = make(x, x.sizes()), dw = weight_grad(w, si == 1), db, ws;
+  if (a.i64(5)) db = make(x, {O});
+  const int64_t bytes = pulsar_fused_linear_backward_workspace_bytes(rows, I, O, (int)act, code(x));
+  if (bytes > 0) ws = make(x, {bytes}, at::kByte);
+  run(pulsar_fused_linear_backward, p(dy), p(x), xs, p(w), so, si, p(pre), q(dx), q(dw),
+      db.defined() ? q(db) : nullptr, rows, I, O, (int)act, code(x), const_cast<void*>(p(ws)),
+      stream(x));
+  return triple(dx, dw, db, true);
+}
+
+// (x, weight [E, I, O], offsets, rows, bias, activation, save_pre) -> y or (y, pre)
+PyObject* grouped_linear_forward(const Args& a) {
+  const Tensor &x = a.t(0), &w = a.t(1), &off = a.t(2);
+  const Tensor idx = a.opt(3), b = a.opt(4);
+  const int64_t act = a.i64(5), E = w.size(0), I = w.size(1), O = w.size(2);
+  const int64_t M = idx.defined() ? idx.numel() : x.size(0);
+  int64_t si, so;
+  weight_strides(w, si, so);
+  const int64_t xs = row_stride(x, "x");
+  const c10::DeviceGuard guard(x.device());
+  Tensor pre;
+  if (a.i64(6)) pre = make(x, {M, O});
+  Tensor y = make(x, {M, act == PULSAR_ACT_SWIGLU ? O / 2 : O});
+  run(pulsar_grouped_linear_forward, p(x), xs, x.size(0), p<int32_t>(idx), p<int32_t>(off), p(w),
+      w.stride(0), si, so, p(b), b.defined() ? code(b) : 0, q(y),
+      pre.defined() ? q(pre) : nullptr, M, E, I, O, (int)act, code(x), stream(x));
+  return pre.defined() ? pair(y, pre, false) : out(y);
+}
+
+// (dy, x, weight [E, I, O], offsets, rows, pre, activation, bias) -> [dx, dw, db]
+PyObject* grouped_linear_backward(const Args& a) {
+  const Tensor &dy = a.t(0), &x = a.t(1), &w = a.t(2), &off = a.t(3);
+  const Tensor idx = a.opt(4), pre = a.opt(5);
+  const int64_t act = a.i64(6), E = w.size(0), I = w.size(1), O = w.size(2), M = dy.size(0);
+  int64_t si, so;
+  weight_strides(w, si, so);
+  const int64_t xs = row_stride(x, "x");
+  const c10::DeviceGuard guard(x.device());
+  // the library writes dw with the input dimension contiguous where the weight's is
+  Tensor dx = make(x, {M, I}), dw = weight_grad(w, si != 1), db, ws;
+  if (a.i64(7)) db = make(x, {E, O});
+  const int64_t bytes =
+      pulsar_grouped_linear_backward_workspace_bytes(M, E, I, O, (int)act, code(x));
+  if (bytes > 0) ws = make(x, {bytes}, at::kByte);
+  run(pulsar_grouped_linear_backward, p(dy), p(x), xs, x.size(0), p<int32_t>(idx), p<int32_t>(off),
+      p(w), w.stride(0), si, so, p(pre), q(dx), q(dw), db.defined() ? q(db) : nullptr, M, E, I, O,
+      (int)act, code(x), const_cast<void*>(p(ws)), stream(x));
+  return triple(dx, dw, db, true);
+}
+
 template <PyObject* (*F)(const Args&), int N>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -333,7 +473,10 @@ PyMethodDef methods[] = {
     OP(qk_rmsnorm_rope_backward, 16), OP(fused_attn_gate_backward, 3),
     OP(fused_swiglu_backward, 3),    OP(causal_conv1d_k4_backward, 3),
     OP(moe_router_topk_backward, 6), OP(moe_dispatch_backward, 5),
-    OP(moe_combine_backward, 5),     {nullptr, nullptr, 0, nullptr}};
+    OP(moe_combine_backward, 5),     OP(moe_group_rows, 2),
+    OP(fused_linear_forward, 6),     OP(fused_linear_backward, 6),
+    OP(grouped_linear_forward, 7),   OP(grouped_linear_backward, 8),
+    {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods};
 

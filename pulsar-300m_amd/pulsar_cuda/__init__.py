@@ -7,7 +7,9 @@ RuntimeError (the reference's TORCH_CHECK). Work is enqueued on torch's current 
 Beyond the reference, every op also accepts fp32 activations.
 
 The forward ops of the decode path and the backward ops of the training path through
-model.forward are provided; the loss (softcapped cross-entropy) and optimizer ops are not
+model.forward are provided, and beyond the reference's module the products between them: the
+dense ones with their epilogue (``fused_linear_*``) and the routed experts' over every
+assignment (``moe_group_rows``, ``grouped_linear_*``). The loss (softcapped cross-entropy) and optimizer ops are not
 part of this module.
 """
 
@@ -16,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import PULSAR_BF16, PULSAR_F32, load_ops
+from ._lib import ACTIVATIONS, PULSAR_BF16, PULSAR_F32, load_ops
 
 __all__ = [
     "rmsnorm_forward", "rope_forward", "qk_rmsnorm_rope_forward", "fused_attn_gate_forward",
@@ -25,6 +27,8 @@ __all__ = [
     "rmsnorm_backward", "qk_rmsnorm_rope_backward", "fused_attn_gate_backward",
     "causal_depthwise_conv1d_k4_backward", "fused_swiglu_backward", "moe_router_topk_backward",
     "moe_dispatch_backward", "moe_combine_backward",
+    "moe_group_rows", "grouped_linear_forward", "grouped_linear_backward",
+    "fused_linear_forward", "fused_linear_backward",
 ]
 
 _LIB = _lib.load()
@@ -415,3 +419,158 @@ def moe_combine_backward(d_routed_out: torch.Tensor, expert_outputs: torch.Tenso
     w = topk_weights.to(torch.bfloat16).contiguous()
     d_eo, d_w = _OPS.moe_combine_backward(d_routed_out, expert_outputs, topk_idx, w, token_to_slot)
     return [d_eo, d_w.to(topk_weights.dtype)]
+
+
+# ---------------------------------------------------------------------------
+# Products with their epilogues, dense and ragged
+# ---------------------------------------------------------------------------
+
+def _act_code(activation: str, d_out: int) -> int:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    if activation == "swiglu" and d_out % 2:
+        raise RuntimeError(f"swiglu needs an even number of output columns, got {d_out}")
+    return code
+
+
+def _operand(t: torch.Tensor, name: str, x: torch.Tensor) -> None:
+    """A tensor of x's dtype on x's device."""
+    _cuda(t, name)
+    _req(t.device == x.device, f"{name} must be on the device of x")
+    _req(t.dtype == x.dtype, f"{name} must have the dtype of x")
+
+
+def _bias(bias, x: torch.Tensor, shape: tuple):
+    if bias is None:
+        return None
+    _cuda(bias, "bias")
+    _req(bias.device == x.device, "bias must be on the device of x")
+    _req(bias.dtype in (x.dtype, torch.float32), "bias must have the dtype of x or be float32")
+    _req(tuple(bias.shape) == shape, f"bias must be {list(shape)}, got {list(bias.shape)}")
+    return bias.contiguous()
+
+
+def _index(t: torch.Tensor, name: str, x: torch.Tensor) -> torch.Tensor:
+    _cuda(t, name)
+    _req(t.device == x.device, f"{name} must be on the device of x")
+    _req(t.dtype == torch.int32 and t.dim() == 1, f"{name} must be 1-dimensional int32")
+    return t.contiguous()
+
+
+def moe_group_rows(topk_idx: torch.Tensor, num_experts: int):
+    """The plan of the routed experts' products over every assignment of topk_idx [N, K] int64,
+    sorted by expert (stable): (offsets int32 [E+1], rows int32 [N*K], slots int32 [N, K]).
+
+    Rows offsets[e] .. offsets[e+1] - 1 belong to expert e, rows[i] is the token of row i and
+    slots[n, k] the row of token n's k-th assignment. Ids outside [0, E) (padding) take no row:
+    slot -1; rows past offsets[E] hold -1. E <= 1024. Nothing is read back to the host.
+
+    The combine of the rows takes the slots as they are, all rows as one expert's:
+    ``moe_combine_forward(y[None], torch.zeros_like(topk_idx), w, slots, shared)``."""
+    _cuda(topk_idx, "topk_idx")
+    _req(topk_idx.dtype == torch.int64, "topk_idx must be int64")
+    _req(topk_idx.dim() == 2 and topk_idx.shape[1] > 0, "topk_idx must be [N, K]")
+    if not 0 < num_experts <= 1024:
+        raise RuntimeError(f"moe_group_rows supports 1 <= E <= 1024, got {num_experts}")
+    return _OPS.moe_group_rows(topk_idx.contiguous(), num_experts)
+
+
+def _linear_operands(x: torch.Tensor, weight: torch.Tensor):
+    _cuda(x, "x")
+    _dtype_code(x, "x")
+    _operand(weight, "weight", x)
+    _req(weight.dim() == 2, "weight must be [d_out, d_in]")
+    _req(x.dim() >= 1 and x.shape[-1] == weight.shape[1], "x must be [..., d_in]")
+    _req(weight.shape[0] > 0 and weight.shape[1] > 0, "weight must not be empty")
+
+
+def fused_linear_forward(x: torch.Tensor, weight: torch.Tensor, bias=None,
+                         activation: str = "none", residual=None, save_pre: bool = False):
+    """act(x @ weight.T + bias) + residual in one launch: x [..., d_in], weight [d_out, d_in]
+    (torch.nn.Linear's; either of its dimensions may be the contiguous one).
+
+    activation: none, relu, silu, gelu (erf), gelu_tanh, sigmoid or swiglu (d_out / 2 columns:
+    silu of the first half times the second, as fused_swiglu_forward). bias in x's dtype or
+    fp32. Sums, bias, activation and residual are fp32, rounded once. x and residual may be
+    2-dimensional with any row stride. save_pre: also returns the values the activation took,
+    [..., d_out], which fused_linear_backward needs for every activation but none."""
+    _linear_operands(x, weight)
+    d_out = weight.shape[0]
+    act = _act_code(activation, d_out)
+    bias = _bias(bias, x, (d_out,))
+    if residual is not None:
+        _operand(residual, "residual", x)
+        cols = d_out // 2 if activation == "swiglu" else d_out
+        _req(residual.shape[:-1] == x.shape[:-1] and residual.dim() == x.dim()
+             and residual.shape[-1] == cols, f"residual must be [..., {cols}]")
+    return _OPS.fused_linear_forward(x, weight, bias, residual, act, int(save_pre))
+
+
+def _saved(dy: torch.Tensor, x: torch.Tensor, pre, lead: tuple, d_out: int, activation: str):
+    cols = d_out // 2 if activation == "swiglu" else d_out
+    _operand(dy, "dy", x)
+    _req(tuple(dy.shape) == (*lead, cols), f"dy must be {[*lead, cols]}, got {list(dy.shape)}")
+    if activation == "none":
+        return None
+    _req(pre is not None, f"pre is needed for activation {activation}")
+    _operand(pre, "pre", x)
+    _req(tuple(pre.shape) == (*lead, d_out), f"pre must be {[*lead, d_out]}, got {list(pre.shape)}")
+    return pre.contiguous()
+
+
+def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre=None,
+                          activation: str = "none", bias: bool = False):
+    """[dx, dweight, dbias] of fused_linear_forward; dbias [d_out] in x's dtype when bias, else
+    None. The residual's gradient is dy. pre: the forward's (unused with activation none).
+    dweight has weight's order of dimensions in memory. act'(pre) dy is rounded to x's dtype,
+    which the matrix cores take, before its products and sums."""
+    _linear_operands(x, weight)
+    act = _act_code(activation, weight.shape[0])
+    pre = _saved(dy, x, pre, tuple(x.shape[:-1]), weight.shape[0], activation)
+    return _OPS.fused_linear_backward(dy.contiguous(), x, weight, pre, act, int(bias))
+
+
+def _grouped_operands(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, rows):
+    _cuda(x, "x")
+    _dtype_code(x, "x")
+    _operand(weight, "weight", x)
+    _req(weight.dim() == 3, "weight must be [E, d_in, d_out]")
+    E, d_in, d_out = weight.shape
+    _req(x.dim() == 2 and x.shape[1] == d_in, "x must be [R, d_in]")
+    _req(E > 0 and d_in > 0 and d_out > 0, "weight must not be empty")
+    offsets = _index(offsets, "offsets", x)
+    _req(offsets.numel() == E + 1, "offsets must have E + 1 elements")
+    return offsets, None if rows is None else _index(rows, "rows", x)
+
+
+def grouped_linear_forward(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
+                           rows=None, bias=None, activation: str = "none",
+                           save_pre: bool = False):
+    """act(x[rows[i]] @ weight[e] + bias[e]) for every row i of every group e, rows
+    offsets[e] .. offsets[e+1] - 1, in one launch: x [R, d_in] (any row stride), weight
+    [E, d_in, d_out] (either of the last two dimensions may be the contiguous one), offsets
+    int32 [E+1] rising from 0, rows int32 [M] (None: row i of x itself, M = R). Returns
+    [M, d_out] (swiglu: d_out / 2). Rows past offsets[E] are zeros, and so is a row of x that
+    an index outside it names. Activations, bias and save_pre as fused_linear_forward's, bias
+    [E, d_out]."""
+    offsets, rows = _grouped_operands(x, weight, offsets, rows)
+    E, _, d_out = weight.shape
+    act = _act_code(activation, d_out)
+    bias = _bias(bias, x, (E, d_out))
+    return _OPS.grouped_linear_forward(x, weight, offsets, rows, bias, act, int(save_pre))
+
+
+def grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                            offsets: torch.Tensor, rows=None, pre=None,
+                            activation: str = "none", bias: bool = False):
+    """[dx, dweight, dbias] of grouped_linear_forward. dx [M, d_in] has a row for each row i (zero
+    past offsets[E]): the gradient of a row of x that several rows name is their sum, with
+    moe_group_rows' plan ``moe_dispatch_backward(dx[None], torch.zeros_like(topk_idx), slots,
+    N, d_in)``. dweight is zero for groups without rows; dbias [E, d_out] when bias."""
+    offsets, rows = _grouped_operands(x, weight, offsets, rows)
+    M = x.shape[0] if rows is None else rows.numel()
+    act = _act_code(activation, weight.shape[2])
+    pre = _saved(dy, x, pre, (M,), weight.shape[2], activation)
+    return _OPS.grouped_linear_backward(dy.contiguous(), x, weight, offsets, rows, pre, act,
+                                        int(bias))

@@ -10,6 +10,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpulsar_h
 PULSAR_OK = 0
 PULSAR_F32 = 0
 PULSAR_BF16 = 1
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5,
+               "swiglu": 6}
 MAX_LAYERS = 16
 
 BUF_TOKENS = 0
@@ -113,6 +115,22 @@ _PROTOS = {
                                         _c_i64, _c_i64, _c_i64, _vp],
     "pulsar_causal_conv1d_k4_backward": [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64,
                                          ctypes.c_int, _vp],
+    "pulsar_moe_group_rows_workspace_bytes": [_c_i64] * 3,
+    "pulsar_moe_group_rows": [_vp] * 4 + [_c_i64] * 3 + [_vp, _vp],
+    "pulsar_fused_linear_forward": [_vp, _c_i64, _vp, _c_i64, _c_i64, _vp, ctypes.c_int, _vp,
+                                    _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+                                    ctypes.c_int, _vp],
+    "pulsar_fused_linear_backward_workspace_bytes": [_c_i64] * 3 + [ctypes.c_int] * 2,
+    "pulsar_fused_linear_backward": [_vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
+                                     _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, _vp,
+                                     _vp],
+    "pulsar_grouped_linear_forward": [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64,
+                                      _vp, ctypes.c_int, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                      ctypes.c_int, ctypes.c_int, _vp],
+    "pulsar_grouped_linear_backward_workspace_bytes": [_c_i64] * 4 + [ctypes.c_int] * 2,
+    "pulsar_grouped_linear_backward": [_vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64,
+                                       _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                       ctypes.c_int, ctypes.c_int, _vp, _vp],
     "pulsar_engine_create": [ctypes.POINTER(PulsarModelDesc), ctypes.POINTER(PulsarEngineConfig),
                              ctypes.POINTER(_vp)],
     "pulsar_engine_destroy": [_vp],
@@ -133,7 +151,10 @@ _PROTOS = {
                                   _vp],
 }
 # entries whose result is not an int status
-_RESTYPES = {"pulsar_sample_workspace_bytes": _c_i64, "pulsar_moe_router_workspace_bytes": _c_i64}
+_RESTYPES = {name: _c_i64 for name in (
+    "pulsar_sample_workspace_bytes", "pulsar_moe_router_workspace_bytes",
+    "pulsar_moe_group_rows_workspace_bytes", "pulsar_fused_linear_backward_workspace_bytes",
+    "pulsar_grouped_linear_backward_workspace_bytes")}
 
 EXPORTED = tuple(["pulsar_last_error", *_PROTOS])
 
