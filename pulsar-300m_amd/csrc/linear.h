@@ -43,19 +43,25 @@ struct LinearArgs {
   int max_tiles;           // products: bound of the row tiles
 };
 
-// The activation of v, and its derivative. expf / erff / tanhf: the fp32 kernels' outputs are
-// held to fp32 rounding.
+// Sigmoid by the exponential and reciprocal instructions: each within one step of fp32, the
+// argument's scaling to base 2 within |v| half steps, so that v sigmoid(v) is off by at most
+// (3 + v^2 e^-|v|) half steps.
+__device__ __forceinline__ float fast_sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504f));
+}
+
+// The activation of v, and its derivative.
 __device__ __forceinline__ float act_value(int act, float v) {
   switch (act) {
     case PULSAR_ACT_RELU: return v < 0.f ? 0.f : v;  // NaN stays NaN
-    case PULSAR_ACT_SILU: return v * sigmoidf_(v);
+    case PULSAR_ACT_SILU: return v * fast_sigmoid(v);
     case PULSAR_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678f));
     case PULSAR_ACT_GELU_TANH: {
       // 0.5 (1 + tanh(u)) = sigmoid(2 u)
       const float u = 0.79788456f * (v + 0.044715f * v * v * v);
-      return v * sigmoidf_(2.f * u);
+      return v * fast_sigmoid(2.f * u);
     }
-    case PULSAR_ACT_SIGMOID: return sigmoidf_(v);
+    case PULSAR_ACT_SIGMOID: return fast_sigmoid(v);
     default: return v;
   }
 }
@@ -67,20 +73,20 @@ __device__ __forceinline__ float act_slope(int act, float v) {
     case PULSAR_ACT_RELU: return v > 0.f ? 1.f : (v <= 0.f ? 0.f : v);
     case PULSAR_ACT_SILU: {
       v = hold(v, 100.f);
-      const float s = sigmoidf_(v);
+      const float s = fast_sigmoid(v);
       return s * (1.f + v * (1.f - s));
     }
     case PULSAR_ACT_GELU:
       v = hold(v, 30.f);
-      return 0.5f * (1.f + erff(v * 0.70710678f)) + v * 0.39894228f * expf(-0.5f * v * v);
+      return 0.5f * (1.f + erff(v * 0.70710678f)) + v * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * v * v);
     case PULSAR_ACT_GELU_TANH: {
       v = hold(v, 30.f);
       const float v2 = v * v;
-      const float s = sigmoidf_(1.59576912f * v * (1.f + 0.044715f * v2));
+      const float s = fast_sigmoid(1.59576912f * v * (1.f + 0.044715f * v2));
       return s + v * s * (1.f - s) * 1.59576912f * (1.f + 0.134145f * v2);
     }
     case PULSAR_ACT_SIGMOID: {
-      const float s = sigmoidf_(v);
+      const float s = fast_sigmoid(v);
       return s * (1.f - s);
     }
     default: return 1.f;

@@ -3,390 +3,16 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "linear.h"
+#include "linear_device.h"
 
 namespace pulsar {
 
 namespace {
 
-constexpr int kXcds = 8;  // consecutive workgroups go to the 8 XCDs in turn
-
-// Operand chunks that lie outside a matrix (past the last k, outside a group, rows an index
-// does not name) are loaded from here: both factors of a product past the end are then zero,
-// whatever the memory beside the matrix holds.
-__device__ __attribute__((aligned(16))) const uint4 kZeroChunk = {0u, 0u, 0u, 0u};
-
-// A workgroup of WR x WC waves owns a tile of BM = 16 RT WR rows and BN = 16 CT WC columns;
-// wave (wr, wc) computes RT x CT matrix-core tiles of 16 x 16.
-template <int RT_, int CT_, int WR_, int WC_>
-struct LinShape {
-  static constexpr int RT = RT_, CT = CT_, WR = WR_, WC = WC_;
-  static constexpr int kThreads = 64 * WR * WC;
-  static constexpr int BM = 16 * RT * WR, BN = 16 * CT * WC;
-};
-
-// How a fragment's lane index i (0..15) of tile t maps to the row of the operand's LDS tile.
-//   PLAIN: 16 t + i.
-//   WIDE (bf16, k contiguous): tiles in pairs, 32 (t / 2) + 8 (i / 4) + 4 (t % 2) + i % 4, so
-//     that a lane ends with 8 consecutive columns of C in the pair's accumulators.
-//   BLOCK (fp32, k strided): B = 4 or 2 tiles share each LDS read, 16 B (t / B) + B i + t % B.
-enum Map { PLAIN, WIDE, BLOCK };
-
-// Stages one operand's tile of R rows x 128 bytes of k (64 bf16 or 32 fp32) in LDS.
-//   KC (k contiguous in memory): LDS [R][8] chunks of 16 bytes; chunk c of row r sits at
-//     c ^ key(r), which spreads the 16 rows a fragment read takes over the banks.
-//   otherwise (rows of R contiguous elements per k): LDS [k][R]. bf16 tiles are read through
-//     the LDS transpose load, 4 k rows x 32 bytes per 16 lanes: 32-byte pairs of chunks sit
-//     at pair ^ (k & 3), which puts the 4 rows on different banks.
-template <typename T, int R, bool KC, Map MAP, int THREADS>
-struct Operand {
-  static constexpr int EV = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
-  static constexpr int kChunks = R * 8, NCH = kChunks / THREADS;
-  static_assert(kChunks % THREADS == 0, "whole chunks per thread");
-  static_assert(KC ? (THREADS / 8) % 16 == 0 : (THREADS * EV / R) % 4 == 0, "one swizzle key per thread");
-
-  const T* base[KC ? NCH : 1];
-  int64_t ld;             // !KC: elements from k to k + 1
-  const int32_t* k_rows;  // !KC: stored row of each k (nullptr: k itself)
-  int64_t k_nrows;
-  uint32_t ok;            // KC: rows that exist
-  int off;                // KC: first k of this thread's chunks; else: its first k row
-  int valid;              // !KC: elements of this thread's chunk columns inside the matrix
-
-  __device__ __forceinline__ static int key(int r) {
-    if constexpr (MAP == WIDE) return (r & 3) | ((r >> 3 & 1) << 2);
-    return r & 7;
-  }
-  // KC: row(local) -> pointer to the stored row, or nullptr
-  template <typename F>
-  __device__ __forceinline__ void init_kc(F&& row) {
-    const int r0 = (int)threadIdx.x >> 3;
-    off = (((int)threadIdx.x & 7) ^ key(r0)) * EV;
-    ok = 0;
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      base[i] = row(r0 + i * (THREADS / 8));
-      ok |= (base[i] ? 1u : 0u) << i;
-    }
-  }
-  // !KC: col(local) -> stored column of the first element, and the columns' end in `lim`
-  template <typename F>
-  __device__ __forceinline__ void init_nc(const T* p, int64_t ld_, const int32_t* rows,
-                                          int64_t nrows, F&& col) {
-    const int c = (int)threadIdx.x % (R / EV);
-    off = (int)threadIdx.x / (R / EV);
-    int lc = c;
-    if constexpr (sizeof(T) == 2) lc = (((c >> 1) ^ (off & 3)) << 1) | (c & 1);
-    int lim;
-    const int g = col(lc * EV, lim);
-    valid = min(max(lim - g, 0), EV);
-    base[0] = p + (valid > 0 ? g : 0);
-    ld = ld_;
-    k_rows = rows;
-    k_nrows = nrows;
-  }
-  // Address and number of elements of chunk i at k step k0 of a matrix with K k's.
-  __device__ __forceinline__ const T* chunk(int i, int k0, int K, int& n) const {
-    if constexpr (KC) {
-      const int k = k0 + off;
-      n = (ok >> i & 1) ? min(max(K - k, 0), EV) : 0;
-      return base[i] + k;
-    } else {
-      const int k = k0 + off + i * (THREADS * EV / R);
-      n = k < K ? valid : 0;
-      int64_t r = k;
-      if (k_rows) {
-        r = k < K ? k_rows[k] : 0;
-        if (r < 0 || r >= k_nrows) n = 0;
-      }
-      return base[0] + r * ld;
-    }
-  }
-  // Direct loads: 16-byte aligned chunks, each whole or absent.
-  __device__ __forceinline__ void fetch(int k0, int K, uint4* lds) const {
-    const int w = (int)threadIdx.x & ~63;
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      int n;
-      const T* p = chunk(i, k0, K, n);
-      load_lds16(n > 0 ? (const void*)p : (const void*)&kZeroChunk, lds + w + i * THREADS);
-    }
-  }
-  // Any alignment: through registers, the partial chunk of a row's end element by element.
-  __device__ __forceinline__ void load(int k0, int K, uint4 (&r)[NCH]) const {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      int n;
-      const T* p = chunk(i, k0, K, n);
-      r[i] = uint4{0u, 0u, 0u, 0u};
-      if (n == EV) {
-        __builtin_memcpy(&r[i], p, 16);
-      } else if (n > 0) {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int e = 0; e < EV; ++e) {
-          if (e >= n) continue;
-          if constexpr (sizeof(T) == 2)
-            w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
-          else
-            w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-        }
-        r[i] = uint4{w[0], w[1], w[2], w[3]};
-      }
-    }
-  }
-  __device__ __forceinline__ void store(const uint4 (&r)[NCH], uint4* lds) const {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) lds[threadIdx.x + i * THREADS] = r[i];
-  }
-};
-
-// Local row of lane index i of tile t.
-template <Map MAP, int BW>
-__device__ __forceinline__ constexpr int map_row(int t, int i) {
-  if (MAP == WIDE) return 32 * (t / 2) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
-  if (MAP == BLOCK) return 16 * BW * (t / BW) + BW * i + t % BW;
-  return 16 * t + i;
-}
-
-template <typename T>
-struct Frag;
-template <>
-struct Frag<bf16> { typedef lin_bf16x8 type; };
-template <>
-struct Frag<float> { typedef lin_f32x4 type; };
-
-// Fragments of NT tiles whose rows start at `row0` of the staged tile, k half s: of bf16 the
-// lane's 8 k's 32 s + 8 (lane / 16) .., of fp32 its 4 k's 16 s + 4 (lane / 16) ...
-template <typename T, int R, bool KC, Map MAP, int BW, int NT>
-__device__ __forceinline__ void read_frags(const uint4* lds, int row0, int s,
-                                           typename Frag<T>::type* f) {
-  const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
-  if constexpr (KC) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int r = row0 + map_row<MAP, BW>(t, i16);
-      const int key = MAP == WIDE ? (r & 3) | ((r >> 3 & 1) << 2) : r & 7;
-      f[t] = __builtin_bit_cast(typename Frag<T>::type, lds[r * 8 + ((4 * s + kq) ^ key)]);
-    }
-  } else if constexpr (sizeof(T) == 2) {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef short s8 __attribute__((ext_vector_type(8)));
-    typedef __attribute__((address_space(3))) s4* lds_s4;
-    // lane j of a 16-lane group addresses k row j / 4, columns 4 (j % 4) ..; it receives
-    // column j of the 4 rows
-    const int k = 32 * s + 8 * kq + (i16 >> 2);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int col = row0 + 16 * t + 4 * (i16 & 3);  // first of 4
-      const int chunk = (((col >> 4) ^ (k & 3)) << 1) | (col >> 3 & 1);
-      const char* p = reinterpret_cast<const char*>(lds) + k * (R * 2) + chunk * 16 + (col & 4) * 2;
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
-      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * (R * 2)));
-      f[t] = __builtin_bit_cast(lin_bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-  } else {
-    const float* l = reinterpret_cast<const float*>(lds);
-#pragma unroll
-    for (int t = 0; t < NT; t += BW)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float* p = l + (16 * s + 4 * kq + j) * R + row0 + 16 * t + BW * i16;
-        if constexpr (BW == 4) {
-          const lin_f32x4 v = *reinterpret_cast<const lin_f32x4*>(p);
-#pragma unroll
-          for (int b = 0; b < 4; ++b) f[t + b][j] = v[b];
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(p);
-          f[t][j] = v.x;
-          f[t + 1][j] = v.y;
-        }
-      }
-  }
-}
-
-__device__ __forceinline__ lin_f32x4 mma(lin_bf16x8 a, lin_bf16x8 b, lin_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ lin_f32x4 mma(lin_f32x4 a, lin_f32x4 b, lin_f32x4 c) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-  return c;
-}
-
-// The main loop: acc += A tile . B tile^T over K. B goes in as the matrix core's first operand,
-// so that a lane ends with 4 consecutive n of its own m. VEC: direct global-to-LDS loads one
-// step ahead in two buffers; otherwise through registers.
-template <typename T, bool VEC, typename SH, typename OA, typename OB, typename F>
-__device__ __forceinline__ void main_loop(const OA& oa, const OB& ob, int K, uint4* sA, uint4* sB,
-                                          F&& compute) {
-  constexpr int BK = OA::BK;
-  const int steps = (K + BK - 1) / BK;
-  if (steps == 0) return;
-  if constexpr (VEC) {
-    oa.fetch(0, K, sA);
-    ob.fetch(0, K, sB);
-    wait_vmcnt<0>();
-    lds_barrier();
-    for (int kt = 0; kt < steps; ++kt) {
-      const int b = kt & 1;
-      if (kt + 1 < steps) {
-        oa.fetch((kt + 1) * BK, K, sA + (b ^ 1) * OA::kChunks);
-        ob.fetch((kt + 1) * BK, K, sB + (b ^ 1) * OB::kChunks);
-      }
-      compute(sA + b * OA::kChunks, sB + b * OB::kChunks);
-      wait_vmcnt<0>();
-      lds_barrier();
-    }
-  } else {
-    uint4 ra[OA::NCH], rb[OB::NCH];
-    oa.load(0, K, ra);
-    ob.load(0, K, rb);
-    oa.store(ra, sA);
-    ob.store(rb, sB);
-    __syncthreads();
-    for (int kt = 0; kt < steps; ++kt) {
-      const int b = kt & 1;
-      if (kt + 1 < steps) {
-        oa.load((kt + 1) * BK, K, ra);
-        ob.load((kt + 1) * BK, K, rb);
-      }
-      compute(sA + b * OA::kChunks, sB + b * OB::kChunks);
-      if (kt + 1 < steps) {
-        oa.store(ra, sA + (b ^ 1) * OA::kChunks);
-        ob.store(rb, sB + (b ^ 1) * OB::kChunks);
-      }
-      __syncthreads();
-    }
-  }
-}
-
-// Rows [r0, r1) of group g, kept inside the matrix whatever the offsets hold; group `groups` is
-// the rows past the last one.
-__device__ __forceinline__ void group_span(const LinearArgs& a, int g, int& r0, int& r1) {
-  if (!a.offsets) {
-    r0 = 0;
-    r1 = g == 0 ? a.rows : 0;
-    return;
-  }
-  r0 = min(max(a.offsets[g], 0), a.rows);
-  r1 = g < a.groups ? min(max(a.offsets[g + 1], 0), a.rows) : a.rows;
-}
-
-// Row tile t of the launch, tiles counted group by group: its group and first row. 64 groups at a
-// time, one per lane. Returns the number of row tiles (t < 0: only that).
-template <int BM>
-__device__ __forceinline__ int find_tile(const LinearArgs& a, int t, int& group, int& r0, int& r1) {
-  const int lane = (int)threadIdx.x & 63;
-  int before = 0;
-  for (int g0 = 0; g0 <= a.groups; g0 += 64) {
-    const int g = g0 + lane;
-    int s0 = 0, s1 = 0;
-    if (g <= a.groups) group_span(a, g, s0, s1);
-    const int nt = s1 > s0 ? (s1 - s0 + BM - 1) / BM : 0;
-    int incl = nt;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += v;
-    }
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (t >= before && t < before + total) {
-      // the first lane whose inclusive count passes t
-      const int src = (int)__builtin_popcountll(__ballot(before + incl <= t));
-      const int first = __builtin_amdgcn_readlane(incl - nt, src);
-      group = g0 + src;
-      r1 = __builtin_amdgcn_readlane(s1, src);
-      r0 = __builtin_amdgcn_readlane(s0, src) + (t - before - first) * BM;
-      return 0;
-    }
-    before += total;
-  }
-  return before;
-}
-
-// Tiles in the order that shares operands through one L2: the launch's tiles are cut into 8
-// contiguous ranges, one per XCD (workgroup L runs on XCD L % 8), and run in bands of kBand
-// rows of tiles, rows fastest: the 32 CUs of an XCD then work on about 8 x 4 tiles.
-constexpr int kBand = 8;
-__device__ __forceinline__ bool place_tile(int tiles_r, int tiles_c, int& tr, int& tc) {
-  const int total = tiles_r * tiles_c;
-  const int L = (int)blockIdx.x, xcd = L % kXcds, slot = L / kXcds;
-  const int per = (total + kXcds - 1) / kXcds;
-  const int item = xcd * per + slot;
-  if (slot >= per || item >= total) return false;
-  const int band = item / (kBand * tiles_c), in = item - band * kBand * tiles_c;
-  const int rows = min(kBand, tiles_r - band * kBand);
-  tr = band * kBand + in % rows;
-  tc = in / rows;
-  return true;
-}
-
-// W consecutive elements, whole or up to n of them.
-template <int W>
-__device__ __forceinline__ void store_run(float* p, const float* v, int n) {
-  if (n >= W) {
-    __builtin_memcpy(p, v, 4 * W);
-  } else {
-#pragma unroll
-    for (int q = 0; q < W; ++q)
-      if (q < n) p[q] = v[q];
-  }
-}
-template <int W>
-__device__ __forceinline__ void store_run(bf16* p, const float* v, int n) {
-  if (n >= W) {
-    uint32_t w[W / 2];
-#pragma unroll
-    for (int q = 0; q < W / 2; ++q)
-      w[q] = (uint32_t)f2bf(v[2 * q]).u | ((uint32_t)f2bf(v[2 * q + 1]).u << 16);
-    __builtin_memcpy(p, w, 2 * W);
-  } else {
-#pragma unroll
-    for (int q = 0; q < W; ++q)
-      if (q < n) p[q] = f2bf(v[q]);
-  }
-}
-template <int W, typename T>
-__device__ __forceinline__ void load_run(const T* p, float* v, int n) {
-  if (n >= W) {
-    T t[W];
-    __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-    for (int q = 0; q < W; ++q) v[q] = to_f(t[q]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < W; ++q) v[q] = q < n ? to_f(p[q]) : 0.f;
-  }
-}
-
-// The n of C that a lane holds, in runs of W consecutive ones: run g, element q is element e of
-// tile t.
-template <Map MAP, int BW>
-struct Runs {
-  static constexpr int W = MAP == WIDE ? 8 : MAP == BLOCK ? BW : 4;
-  __device__ __forceinline__ static constexpr int tile(int g, int q) {
-    return MAP == WIDE ? 2 * g + (q >> 2) : MAP == BLOCK ? BW * (g / 4) + q : g;
-  }
-  __device__ __forceinline__ static constexpr int elem(int g, int q) {
-    return MAP == WIDE ? q & 3 : MAP == BLOCK ? g % 4 : q;
-  }
-  __device__ __forceinline__ static int col(int g, int kq) {
-    return MAP == WIDE ? 32 * g + 8 * kq
-         : MAP == BLOCK ? 16 * BW * (g / 4) + BW * (4 * kq + g % 4)
-                        : 16 * g + 4 * kq;
-  }
-};
-
-template <typename T, bool KC>
-constexpr Map out_map() {
-  return KC ? (sizeof(T) == 2 ? WIDE : PLAIN) : (sizeof(T) == 2 ? PLAIN : BLOCK);
-}
-
 // Products over ragged rows: C[i][n] = epi(sum_k A[row(i)][k] B_group[n][k]). PAIR (SwiGLU): a
 // tile's columns are BN / 2 gate columns and their up-projection twins N / 2 further on.
 template <typename T, bool BKC, bool PAIR, bool VEC, typename SH>
-__global__ void __launch_bounds__(SH::kThreads, 2) linear_rows_kernel(LinearArgs a) {
+__global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(LinearArgs a) {
   constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
   constexpr Map MAP = out_map<T, BKC>();
   constexpr int NCT = PAIR ? CT / 2 : CT;  // tiles of output columns per wave
@@ -394,15 +20,16 @@ __global__ void __launch_bounds__(SH::kThreads, 2) linear_rows_kernel(LinearArgs
   static_assert(MAP == PLAIN || NCT % (MAP == WIDE ? 2 : BW) == 0, "whole runs per wave");
   typedef Operand<T, BM, true, PLAIN, SH::kThreads> OA;
   typedef Operand<T, BN, BKC, MAP, SH::kThreads> OB;
-  __shared__ uint4 sA[2 * OA::kChunks], sB[2 * OB::kChunks];
+  __shared__ uint4 lds[2 * (OA::kChunks + OB::kChunks)];
+  uint4 *sA = lds, *sB = lds + 2 * OA::kChunks;
+  static_assert(sizeof(lds) >= SH::WR * SH::WC * Slab<CT>::kFloats * 4, "the epilogue's slabs fit");
 
   const int f = PAIR ? a.N / 2 : a.N;          // output columns
   constexpr int OBN = PAIR ? BN / 2 : BN;      // output columns of a tile
   const int tiles_c = (f + OBN - 1) / OBN;
   int group = 0, r0 = 0, r1 = 0, tr, tc;
-  const int tiles_r = find_tile<BM>(a, -1, group, r0, r1);
-  if (!place_tile(tiles_r, tiles_c, tr, tc)) return;
-  find_tile<BM>(a, tr, group, r0, r1);
+  if (!place_tile(count_tiles<BM>(a), tiles_c, tr, tc)) return;
+  if (!find_tile<BM>(a, tr, group, r0, r1)) return;
   const int n0 = tc * OBN;
   const bool none = group >= a.groups;  // rows of no group: zeros
   const int K = none ? 0 : a.K;
@@ -443,75 +70,37 @@ __global__ void __launch_bounds__(SH::kThreads, 2) linear_rows_kernel(LinearArgs
 #pragma unroll
     for (int j = 0; j < CT; ++j) acc[i][j] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  main_loop<T, VEC, SH>(oa, ob, K, sA, sB, [&](const uint4* la, const uint4* lb) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      typename Frag<T>::type fa[RT], fb[CT];
-      read_frags<T, BM, true, PLAIN, 1, RT>(la, row_w, s, fa);
-      read_frags<T, BN, BKC, MAP, BW, NCT>(lb, col_w, s, fb);
-      if constexpr (PAIR) read_frags<T, BN, BKC, MAP, BW, NCT>(lb, OBN + col_w, s, fb + NCT);
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+  typedef typename Frag<T>::type F;
+  const Reader<T, BM, true, PLAIN, 1> ra(row_w);
+  const Reader<T, BN, BKC, MAP, BW> rb(col_w), ru(OBN + col_w);
+  auto rd = [&](const uint4* la, const uint4* lb, int s, F(&fa)[RT], F(&fb)[CT], int part) {
+    if (part == 0) {
+      rb.template read<NCT>(lb, s, fb);
+      if constexpr (PAIR) ru.template read<NCT>(lb, s, fb + NCT);
+    } else {
+      ra.template read<RT>(la, s, fa);
     }
-  });
-
-  // epilogue in fp32, one rounding per output
-  typedef Runs<MAP, BW> RN;
-  constexpr int W = RN::W, NG = NCT * 4 / W;
-  T* C = reinterpret_cast<T*>(a.C);
-  T* pre = reinterpret_cast<T*>(a.pre);
-  const T* res = reinterpret_cast<const T*>(a.residual);
+  };
+  if constexpr (VEC) {
+    pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, rd, [](int, F(&)[RT], F(&)[CT]) {});
+  } else {
+    staged_loop<T>(oa, ob, K, sA, sB, [&](const uint4* la, const uint4* lb) {
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int col = n0 + col_w + RN::col(g, kq), n = f - col;
-    if (n <= 0) continue;
-    float bias[2][W];
+      for (int s = 0; s < 2; ++s) {
+        F fa[RT], fb[CT];
+        rd(la, lb, s, fa, fb, 0);
+        rd(la, lb, s, fa, fb, 1);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int q = 0; q < W; ++q) bias[h][q] = 0.f;
-    if (a.bias && !none) {
-#pragma unroll
-      for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
-        const int64_t o = (int64_t)group * a.N + col + h * f;
-        if (a.bias_dtype == PULSAR_F32)
-          load_run<W>(reinterpret_cast<const float*>(a.bias) + o, bias[h], n);
-        else
-          load_run<W>(reinterpret_cast<const bf16*>(a.bias) + o, bias[h], n);
+          for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int64_t r = r0 + row_w + 16 * i + i16;
-      if (r >= r1) continue;
-      float v[W], u[W];
-#pragma unroll
-      for (int q = 0; q < W; ++q) {
-        v[q] = acc[i][RN::tile(g, q)][RN::elem(g, q)] + bias[0][q];
-        u[q] = PAIR ? acc[i][(PAIR ? NCT : 0) + RN::tile(g, q)][RN::elem(g, q)] + bias[1][q] : 0.f;
-      }
-      if (pre) {
-        store_run<W>(pre + r * a.ldpre + col, v, n);
-        if constexpr (PAIR) store_run<W>(pre + r * a.ldpre + f + col, u, n);
-      }
-      if constexpr (PAIR) {
-#pragma unroll
-        for (int q = 0; q < W; ++q) v[q] = v[q] * sigmoidf_(v[q]) * u[q];
-      } else if (a.act != PULSAR_ACT_NONE && !none) {
-#pragma unroll
-        for (int q = 0; q < W; ++q) v[q] = act_value(a.act, v[q]);
-      }
-      if (res) {
-        float x[W];
-        load_run<W>(res + r * a.ldr + col, x, n);
-#pragma unroll
-        for (int q = 0; q < W; ++q) v[q] += x[q];
-      }
-      store_run<W>(C + r * a.ldc + col, v, n);
-    }
+    });
   }
+
+  __syncthreads();  // the tiles' memory now holds the epilogue's rows
+  rows_epilogue<T, MAP, BW, PAIR>(a, acc, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats, group, none,
+                                  r0 + row_w, r1, n0 + col_w, f);
 }
 
 // Weight gradient: C_group[m][n] = sum over the group's rows r of A[r][m] B[r][n], rows through
@@ -519,25 +108,25 @@ __global__ void __launch_bounds__(SH::kThreads, 2) linear_rows_kernel(LinearArgs
 // along, by one more product with ones in the tiles at 0 of the other dimension (0 none, 1 A,
 // 2 B).
 template <typename T, bool VEC, int SIDE, typename SH>
-__global__ void __launch_bounds__(SH::kThreads, 2) linear_wgrad_kernel(LinearArgs a) {
+__global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(LinearArgs a) {
   constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
   constexpr Map MAP = out_map<T, false>();
   constexpr int BWR = RT >= 4 ? 4 : 2, BWC = CT >= 4 ? 4 : 2;
   typedef Operand<T, BM, false, MAP, SH::kThreads> OA;
   typedef Operand<T, BN, false, MAP, SH::kThreads> OB;
-  __shared__ uint4 sA[2 * OA::kChunks], sB[2 * OB::kChunks];
+  __shared__ uint4 lds[2 * (OA::kChunks + OB::kChunks)];
+  uint4 *sA = lds, *sB = lds + 2 * OA::kChunks;
+  static_assert(sizeof(lds) >= SH::WR * SH::WC * Slab<CT>::kFloats * 4, "the epilogue's slabs fit");
 
-  // (group, split, row of tiles) are the rows of the launch's tiles
-  int tr, tc;
-  if (!place_tile(a.groups * a.splits * a.tiles_m, a.tiles_n, tr, tc)) return;
-  const int mt = tr % a.tiles_m, gs = tr / a.tiles_m, split = gs % a.splits, group = gs / a.splits;
+  int group, split, mt, tc;
+  if (!place_wgrad(a, group, split, mt, tc)) return;
   int r0, r1;
   group_span(a, group, r0, r1);
   r1 = max(r0, r1);
   if (a.splits > 1) {
-    const int per = ((r1 - r0 + a.splits - 1) / a.splits + OA::BK - 1) / OA::BK * OA::BK;
-    r0 = min(r0 + split * per, r1);
-    r1 = min(r0 + per, r1);
+    const int64_t per = ((r1 - r0 + a.splits - 1) / a.splits + OA::BK - 1) / OA::BK * OA::BK;
+    r0 = (int)min(r0 + split * per, (int64_t)r1);
+    r1 = (int)min(r0 + per, (int64_t)r1);
   }
   const int m0 = mt * BM, n0 = tc * BN;
   OA oa;
@@ -572,73 +161,47 @@ __global__ void __launch_bounds__(SH::kThreads, 2) linear_wgrad_kernel(LinearArg
     for (int i = 0; i < (SIDE == 1 ? RT : CT); ++i) sum[i] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  main_loop<T, VEC, SH>(oa, ob, r1 - r0, sA, sB, [&](const uint4* la, const uint4* lb) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      typename Frag<T>::type fa[RT], fb[CT];
-      read_frags<T, BM, false, MAP, BWR, RT>(la, row_w, s, fa);
-      read_frags<T, BN, false, MAP, BWC, CT>(lb, col_w, s, fb);
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
-      if constexpr (SIDE == 1) {
-        if (sums)
-#pragma unroll
-          for (int i = 0; i < RT; ++i) sum[i] = mma(ones, fa[i], sum[i]);
-      }
-      if constexpr (SIDE == 2) {
-        if (sums)
-#pragma unroll
-          for (int j = 0; j < CT; ++j) sum[j] = mma(fb[j], ones, sum[j]);
-      }
-    }
-  });
-
-  typedef Runs<MAP, BWC> RN;
-  constexpr int W = RN::W, NG = CT * 4 / W;
-  const int64_t pg = (int64_t)split * a.groups + group;  // a split's partial results
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int col = n0 + col_w + RN::col(g, kq), n = a.N - col;
-    if (n <= 0) continue;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int64_t m = m0 + row_w + map_row<MAP, BWR>(i, i16);
-      if (m >= a.M) continue;
-      float v[W];
-#pragma unroll
-      for (int q = 0; q < W; ++q) v[q] = acc[i][RN::tile(g, q)][RN::elem(g, q)];
-      if (a.splits > 1)
-        store_run<W>(a.part + (pg * a.M + m) * a.N + col, v, n);
-      else
-        store_run<W>(reinterpret_cast<T*>(a.C) + group * a.c_group + m * a.ldc + col, v, n);
+  typedef typename Frag<T>::type F;
+  const Reader<T, BM, false, MAP, BWR> ra(row_w);
+  const Reader<T, BN, false, MAP, BWC> rb(col_w);
+  auto rd = [&](const uint4* la, const uint4* lb, int s, F(&fa)[RT], F(&fb)[CT], int part) {
+    if (part == 0)
+      rb.template read<CT>(lb, s, fb);
+    else
+      ra.template read<RT>(la, s, fa);
+  };
+  auto extra = [&](int i, F(&fa)[RT], F(&fb)[CT]) {
+    if constexpr (SIDE == 1) {
+      if (sums) sum[i] = mma(ones, fa[i], sum[i]);
     }
     if constexpr (SIDE == 2) {
-      if (sums && i16 == 0) {
-        float v[W];
+      if (sums && i == 0)
 #pragma unroll
-        for (int q = 0; q < W; ++q) v[q] = sum[RN::tile(g, q)][RN::elem(g, q)];
-        if (a.splits > 1)
-          store_run<W>(a.part_db + pg * a.N + col, v, n);
-        else
-          store_run<W>(reinterpret_cast<T*>(a.db) + (int64_t)group * a.N + col, v, n);
-      }
+        for (int j = 0; j < CT; ++j) sum[j] = mma(fb[j], ones, sum[j]);
     }
-  }
-  if constexpr (SIDE == 1) {
-    if (sums && kq == 0) {
+  };
+  if constexpr (VEC) {
+    pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, rd, extra);
+  } else {
+    staged_loop<T>(oa, ob, r1 - r0, sA, sB, [&](const uint4* la, const uint4* lb) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const int m = m0 + row_w + map_row<MAP, BWR>(i, i16);
-        if (m >= a.M) continue;
-        if (a.splits > 1)
-          a.part_db[pg * a.M + m] = sum[i][0];
-        else
-          reinterpret_cast<T*>(a.db)[(int64_t)group * a.M + m] = from_f<T>(sum[i][0]);
+      for (int s = 0; s < 2; ++s) {
+        F fa[RT], fb[CT];
+        rd(la, lb, s, fa, fb, 0);
+        rd(la, lb, s, fa, fb, 1);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+#pragma unroll
+          for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+          extra(i, fa, fb);
+        }
       }
-    }
+    });
   }
+
+  __syncthreads();  // the tiles' memory now holds the epilogue's rows
+  wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats,
+                                         sums, group, split, m0 + row_w, n0 + col_w);
 }
 
 // Sums of a weight gradient's splits, in order; `count` elements of one split's partials, the
@@ -681,7 +244,7 @@ __global__ void __launch_bounds__(256) linear_act_grad_kernel(const T* pre, cons
       load_run<W>(pre + r * 2 * f + f + c, u, n);
 #pragma unroll
       for (int q = 0; q < W; ++q) {
-        ou[q] = d[q] * g[q] * sigmoidf_(g[q]);
+        ou[q] = d[q] * g[q] * fast_sigmoid(g[q]);
         o[q] = d[q] * u[q] * act_slope(PULSAR_ACT_SILU, g[q]);
       }
       store_run<W>(dpre + r * 2 * f + c, o, n);
@@ -695,8 +258,9 @@ __global__ void __launch_bounds__(256) linear_act_grad_kernel(const T* pre, cons
   }
 }
 
-typedef LinShape<4, 4, 2, 2> LinLarge;  // 128 x 128
-typedef LinShape<2, 4, 2, 2> LinSmall;  // 64 x 128
+typedef LinShape<8, 4, 2, 4, 2> LinWide;   // 256 x 256
+typedef LinShape<4, 4, 2, 2, 2> LinLarge;  // 128 x 128
+typedef LinShape<2, 4, 2, 2, 2> LinSmall;  // 64 x 128
 
 template <typename T, bool BKC, bool PAIR, bool VEC, typename SH>
 int launch_rows_shape(LinearArgs& a, hipStream_t s) {
@@ -706,6 +270,7 @@ int launch_rows_shape(LinearArgs& a, hipStream_t s) {
       ? a.rows / SH::BM + std::min<int64_t>(a.groups + 1, a.rows)
       : (a.rows + SH::BM - 1) / SH::BM;
   const int64_t tiles = tiles_r * ((f + obn - 1) / obn);
+  a.max_tiles = (int)tiles_r;
   if (tiles > (int64_t)1 << 30) return fail(PULSAR_ERR_INVALID, "linear: launch too large");
   linear_rows_kernel<T, BKC, PAIR, VEC, SH>
       <<<(unsigned)((tiles + kXcds - 1) / kXcds * kXcds), SH::kThreads, 0, s>>>(a);
@@ -720,10 +285,19 @@ int launch_rows(LinearArgs& a, bool b_kc, hipStream_t s) {
   const int f = pair ? a.N / 2 : a.N;
   const bool vec = aligned16(a.A) && aligned16(a.B) && a.lda % ev == 0 && a.ldb % ev == 0 &&
                    a.b_group % ev == 0 && a.K % ev == 0 && (b_kc || f % ev == 0);
-  const int64_t t128 = ((a.rows + 127) / 128) * (((int64_t)a.N + 127) / 128);
+  // the launch's tiles, a ragged group adding half of one on average
+  auto tiles = [&](int r, int c) {
+    return ((a.rows + r - 1) / r + (a.offsets ? a.groups / 2 : 0)) * (((int64_t)a.N + c - 1) / c);
+  };
+  const int64_t t128 = tiles(128, 128), t256 = tiles(256, 256);
+  const double steps = (a.K + 4 * ev * 2 - 1) / (4 * ev * 2);
   const bool large = t128 >= 256;
+  const bool wide = ((t256 + 255) / 256) * (10 + 1.7 * steps) < ((t128 + 511) / 512) * (5.7 + 0.98 * steps);
   auto go = [&](auto kc, auto pr, auto vc) {
     constexpr bool KC = decltype(kc)::value, P = decltype(pr)::value, V = decltype(vc)::value;
+    if constexpr (V && sizeof(T) == 2) {
+      if (wide) return launch_rows_shape<T, KC, P, V, LinWide>(a, s);
+    }
     if (large) return launch_rows_shape<T, KC, P, V, LinLarge>(a, s);
     return launch_rows_shape<T, KC, P, V, LinSmall>(a, s);
   };
@@ -736,35 +310,40 @@ int launch_rows(LinearArgs& a, bool b_kc, hipStream_t s) {
   return b_kc ? pick_pair(std::true_type{}) : pick_pair(std::false_type{});
 }
 
-// Rows of each of a weight gradient's splits: enough workgroups to fill the chip twice where
-// the tiles alone do not, no split shorter than 512 rows. The bound is the average group.
-int wgrad_splits(int64_t rows, int groups, int64_t tiles) {
-  if (tiles >= 384) return 1;
-  const int64_t avg = rows / std::max(groups, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), avg / 512));
-}
-int64_t wgrad_tiles(int64_t d_in, int64_t d_out, int groups) {
-  return ((d_in + 127) / 128) * ((d_out + 127) / 128) * groups;
+// How a weight gradient is cut: tile shape and splits of the sum over rows. Splits: enough
+// workgroups to fill the chip twice where the tiles alone do not, none shorter than 512 rows of
+// an average group.
+struct WgradPlan {
+  bool wide;
+  int splits;
+};
+WgradPlan wgrad_plan(int64_t rows, int64_t groups, int64_t d_in, int64_t d_out, int dtype) {
+  auto tiles = [&](int64_t t) { return ((d_in + t - 1) / t) * ((d_out + t - 1) / t) * groups; };
+  auto splits = [&](int64_t n, int64_t fill) {
+    return (int)std::max<int64_t>(1, std::min(fill / std::max<int64_t>(n, 1), rows / groups / 512));
+  };
+  const int wide = splits(tiles(256), 256);
+#ifndef WGRAD_WIDE
+#define WGRAD_WIDE (groups == 1 && tiles(256) * wide >= 224)
+#endif
+  if (dtype == PULSAR_BF16 && WGRAD_WIDE) return {true, wide};
+  return {false, tiles(128) >= 384 ? 1 : splits(tiles(128), 512)};
 }
 
-template <typename T>
-int launch_wgrad(LinearArgs& a, bool vec, int side, hipStream_t s) {
-  typedef LinLarge SH;
+template <typename T, bool VEC, typename SH>
+int launch_wgrad(LinearArgs& a, int side, hipStream_t s) {
   a.tiles_m = (a.M + SH::BM - 1) / SH::BM;
   a.tiles_n = (a.N + SH::BN - 1) / SH::BN;
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.groups * a.splits;
+  const int64_t per = (int64_t)a.tiles_m * a.tiles_n * a.splits, tiles = per * a.groups;
   if (tiles > (int64_t)1 << 30) return fail(PULSAR_ERR_INVALID, "linear: launch too large");
-  const unsigned grid = (unsigned)((tiles + kXcds - 1) / kXcds * kXcds);
-  auto go = [&](auto v, auto sd) {
-    linear_wgrad_kernel<T, decltype(v)::value, decltype(sd)::value, SH><<<grid, SH::kThreads, 0, s>>>(a);
-  };
-  auto pick = [&](auto v) {
-    if (side == 0) go(v, std::integral_constant<int, 0>{});
-    else if (side == 1) go(v, std::integral_constant<int, 1>{});
-    else go(v, std::integral_constant<int, 2>{});
-  };
-  if (vec) pick(std::true_type{});
-  else pick(std::false_type{});
+  const int64_t run = kXcds * std::max<int64_t>(1, per / kXcds);  // place_wgrad's
+  const unsigned grid = (unsigned)((tiles + run - 1) / run * run);
+  if (side == 0)
+    linear_wgrad_kernel<T, VEC, 0, SH><<<grid, SH::kThreads, 0, s>>>(a);
+  else if (side == 1)
+    linear_wgrad_kernel<T, VEC, 1, SH><<<grid, SH::kThreads, 0, s>>>(a);
+  else
+    linear_wgrad_kernel<T, VEC, 2, SH><<<grid, SH::kThreads, 0, s>>>(a);
   PULSAR_LAUNCH_CHECK();
   if (a.splits > 1) {
     const int64_t n_c = (int64_t)a.groups * a.M * a.N;
@@ -830,7 +409,7 @@ int64_t workspace_bytes(int64_t rows, int64_t groups, int64_t d_in, int64_t d_ou
   if (rows < 0 || groups < 1 || d_in < 1 || d_out < 1) return -1;
   const int64_t es = dtype == PULSAR_BF16 ? 2 : 4;
   const int64_t dpre = act == PULSAR_ACT_NONE ? 0 : (rows * d_out * es + 255) / 256 * 256;
-  const int splits = wgrad_splits(rows, (int)groups, wgrad_tiles(d_in, d_out, (int)groups));
+  const int splits = wgrad_plan(rows, groups, d_in, d_out, dtype).splits;
   const int64_t part = splits > 1 ? splits * groups * (d_in * d_out + d_out) * 4 : 0;
   return dpre + part;
 }
@@ -880,14 +459,19 @@ int backward_t(const void* dy, const void* x, int64_t x_rs, int64_t x_rows, cons
   a.offsets = offsets; a.groups = (int)groups; a.rows = (int)rows;
   a.C = dw; a.ldc = a.N; a.c_group = (int64_t)a.M * a.N;
   a.db = db;
-  a.splits = wgrad_splits(rows, (int)groups, wgrad_tiles(d_in, d_out, (int)groups));
+  const WgradPlan plan = wgrad_plan(rows, groups, d_in, d_out, sizeof(T) == 2 ? PULSAR_BF16 : PULSAR_F32);
+  a.splits = plan.splits;
   if (a.splits > 1) {
     a.part = reinterpret_cast<float*>(ws);
     a.part_db = a.part + (int64_t)a.splits * groups * d_in * d_out;
   }
   const bool vec = aligned16(a.A) && aligned16(a.B) && a.lda % ev == 0 && a.ldb % ev == 0 &&
                    a.M % ev == 0 && a.N % ev == 0;
-  return launch_wgrad<T>(a, vec, db ? (dpre_a ? 1 : 2) : 0, s);
+  const int side = db ? (dpre_a ? 1 : 2) : 0;
+  if constexpr (sizeof(T) == 2) {
+    if (plan.wide && vec) return launch_wgrad<T, true, LinWide>(a, side, s);
+  }
+  return vec ? launch_wgrad<T, true, LinLarge>(a, side, s) : launch_wgrad<T, false, LinLarge>(a, side, s);
 }
 
 int null_check(const char* what) {
