@@ -252,18 +252,27 @@ int pulsar_moe_group_rows(const int64_t* topk_idx, int32_t* offsets, int32_t* ro
  *   x: [rows, d_in], row stride x_rs; w element (o, i) at o w_out + i w_in, one of the strides 1;
  *   bias: [d_out] of bias_dtype, nullable; residual: [rows, columns of y], row stride
  *   residual_rs, nullable; y: contiguous [rows, d_out] (SwiGLU: d_out / 2); pre: contiguous
- *   [rows, d_out], the values the activation took, for the backward call, nullable. */
+ *   [rows, d_out], the values the activation took, for the backward call, nullable.
+ *   workspace: the given number of bytes (-1: bad arguments) of device memory, 16-byte aligned,
+ *   any contents; none when it is 0. Operands whose rows are not made of whole, aligned 16-byte
+ *   chunks are copied into it first (the pointers are only looked at). */
+int64_t pulsar_fused_linear_forward_workspace_bytes(const void* x, int64_t x_rs, const void* w,
+                                                    int64_t w_out, int64_t w_in, int64_t rows,
+                                                    int64_t d_in, int64_t d_out, int activation,
+                                                    int dtype);
 int pulsar_fused_linear_forward(const void* x, int64_t x_rs, const void* w, int64_t w_out,
                                 int64_t w_in, const void* bias, int bias_dtype,
                                 const void* residual, int64_t residual_rs, void* y, void* pre,
                                 int64_t rows, int64_t d_in, int64_t d_out, int activation,
-                                int dtype, hipStream_t stream);
+                                int dtype, void* workspace, hipStream_t stream);
 
 /* Its gradients: dx contiguous [rows, d_in]; dw contiguous in w's own order (w_in == 1:
  * [d_out][d_in], else [d_in][d_out]); db [d_out] in dtype, nullable (not computed). dy
  * contiguous; the residual's gradient is dy. pre: the forward's (unused without activation).
- * workspace: the given number of bytes of device memory, 16-byte aligned, any contents. */
-int64_t pulsar_fused_linear_backward_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out,
+ * workspace as above. */
+int64_t pulsar_fused_linear_backward_workspace_bytes(const void* dy, const void* x, int64_t x_rs,
+                                                     const void* w, int64_t w_out, int64_t w_in,
+                                                     int64_t rows, int64_t d_in, int64_t d_out,
                                                      int activation, int dtype);
 int pulsar_fused_linear_backward(const void* dy, const void* x, int64_t x_rs, const void* w,
                                  int64_t w_out, int64_t w_in, const void* pre, void* dx, void* dw,
@@ -274,19 +283,28 @@ int pulsar_fused_linear_backward(const void* dy, const void* x, int64_t x_rs, co
  *   x: [x_rows, d_in], row stride x_rs; row_index int32 [rows], nullable (row i itself; x_rows
  *   == rows); an index outside x reads as a row of zeros. offsets int32 [groups + 1], rising
  *   from 0 to at most rows; rows past offsets[groups] become zeros in y and pre. w element
- *   (e, i, o) at e w_group + i w_in + o w_out, one of w_in and w_out 1; bias [groups, d_out]. */
+ *   (e, i, o) at e w_group + i w_in + o w_out, one of w_in and w_out 1; bias [groups, d_out].
+ *   workspace as above. */
+int64_t pulsar_grouped_linear_forward_workspace_bytes(const void* x, int64_t x_rs, int64_t x_rows,
+                                                      const void* w, int64_t w_group, int64_t w_in,
+                                                      int64_t w_out, int64_t rows, int64_t groups,
+                                                      int64_t d_in, int64_t d_out, int activation,
+                                                      int dtype);
 int pulsar_grouped_linear_forward(const void* x, int64_t x_rs, int64_t x_rows,
                                   const int32_t* row_index, const int32_t* offsets, const void* w,
                                   int64_t w_group, int64_t w_in, int64_t w_out, const void* bias,
                                   int bias_dtype, void* y, void* pre, int64_t rows,
                                   int64_t groups, int64_t d_in, int64_t d_out, int activation,
-                                  int dtype, hipStream_t stream);
+                                  int dtype, void* workspace, hipStream_t stream);
 
 /* Its gradients: dx contiguous [rows, d_in], a row for each row of y (the sum over the rows that
  * share a row of x is the caller's: pulsar_moe_dispatch_backward), zeros past offsets[groups];
  * dw contiguous in w's own order, groups outermost, zeros for empty groups; db [groups, d_out]
  * in dtype, nullable. */
-int64_t pulsar_grouped_linear_backward_workspace_bytes(int64_t rows, int64_t groups, int64_t d_in,
+int64_t pulsar_grouped_linear_backward_workspace_bytes(const void* dy, const void* x, int64_t x_rs,
+                                                       int64_t x_rows, const void* w,
+                                                       int64_t w_group, int64_t w_in, int64_t w_out,
+                                                       int64_t rows, int64_t groups, int64_t d_in,
                                                        int64_t d_out, int activation, int dtype);
 int pulsar_grouped_linear_backward(const void* dy, const void* x, int64_t x_rs, int64_t x_rows,
                                    const int32_t* row_index, const int32_t* offsets, const void* w,

@@ -21,7 +21,7 @@ OUT = os.path.join(HERE, "pulsar_cuda", "libpulsar_hip.so")
 OPS_OUT = os.path.join(HERE, "pulsar_cuda", "_ops.so")
 BUILD = os.path.join(HERE, "_build")
 SOURCES = ["ops.hip", "gemm.hip", "gemm_wide.hip", "gemm_f32.hip", "rows.hip", "sample.hip", "engine.hip", "backward.hip",
-           "group.hip", "linear.hip"]
+           "group.hip", "linear.hip", "linear_few.hip"]
 ARCH = os.environ.get("PULSAR_HIP_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

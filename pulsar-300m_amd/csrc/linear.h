@@ -26,6 +26,7 @@ struct LinearArgs {
   int groups;
   int rows;                // ragged rows in all
   int M, N, K;             // M: weight gradient only; K: products only
+  int up;                  // SwiGLU: B's first row or column of the up projection
   void* C;
   int64_t ldc, c_group;
   void* pre;               // products: pre-activation values (nullptr: not kept)
@@ -42,6 +43,14 @@ struct LinearArgs {
   int tiles_m, tiles_n;    // weight gradient: tiles of one group
   int max_tiles;           // products: bound of the row tiles
 };
+
+// Products with few rows a group (linear_few.hip), in shapes of 16-row and 16-column tiles of a
+// workgroup (the first not for SwiGLU).
+struct FewShape {
+  int rt, ct;
+};
+constexpr FewShape kFewShapes[6] = {{1, 1}, {1, 2}, {2, 2}, {1, 4}, {2, 4}, {4, 4}};
+int launch_linear_few(LinearArgs& a, int dtype, bool b_kc, int shape, hipStream_t s);
 
 // Sigmoid by the exponential and reciprocal instructions: each within one step of fp32, the
 // argument's scaling to base 2 within |v| half steps, so that v sigmoid(v) is off by at most

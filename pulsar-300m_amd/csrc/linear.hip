@@ -1,6 +1,7 @@
 // Dense and ragged (grouped by expert) products with bias, activation and residual in the
 // epilogue, and their gradients: fused_linear_* and grouped_linear_* of the op surface.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "linear_device.h"
@@ -10,8 +11,8 @@ namespace pulsar {
 namespace {
 
 // Products over ragged rows: C[i][n] = epi(sum_k A[row(i)][k] B_group[n][k]). PAIR (SwiGLU): a
-// tile's columns are BN / 2 gate columns and their up-projection twins N / 2 further on.
-template <typename T, bool BKC, bool PAIR, bool VEC, typename SH>
+// tile's columns are BN / 2 gate columns and their up-projection twins.
+template <typename T, bool BKC, bool PAIR, typename SH>
 __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(LinearArgs a) {
   constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
   constexpr Map MAP = out_map<T, BKC>();
@@ -27,9 +28,8 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
   const int f = PAIR ? a.N / 2 : a.N;          // output columns
   constexpr int OBN = PAIR ? BN / 2 : BN;      // output columns of a tile
   const int tiles_c = (f + OBN - 1) / OBN;
-  int group = 0, r0 = 0, r1 = 0, tr, tc;
-  if (!place_tile(count_tiles<BM>(a), tiles_c, tr, tc)) return;
-  if (!find_tile<BM>(a, tr, group, r0, r1)) return;
+  int tc, group, r0, r1;
+  if (!locate_tile<BM>(a, tiles_c, tc, group, r0, r1)) return;
   const int n0 = tc * OBN;
   const bool none = group >= a.groups;  // rows of no group: zeros
   const int K = none ? 0 : a.K;
@@ -48,15 +48,15 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
   OB ob;
   if constexpr (BKC) {
     ob.init_kc([&](int c) -> const T* {
-      const int64_t n = PAIR ? (c < OBN ? min(n0 + c, f - 1) : f + min(n0 + c - OBN, f - 1))
+      const int64_t n = PAIR ? (c < OBN ? min(n0 + c, f - 1) : a.up + min(n0 + c - OBN, f - 1))
                              : min(n0 + c, f - 1);
       return B + n * a.ldb;
     });
   } else {
     ob.init_nc(B, a.ldb, nullptr, 0, [&](int c, int& lim) {
       const bool up = PAIR && c >= OBN;
-      lim = up ? a.N : f;
-      return up ? f + n0 + c - OBN : n0 + c;
+      lim = up ? a.up + f : f;
+      return up ? a.up + n0 + c - OBN : n0 + c;
     });
   }
 
@@ -81,22 +81,7 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
       ra.template read<RT>(la, s, fa);
     }
   };
-  if constexpr (VEC) {
-    pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, rd, [](int, F(&)[RT], F(&)[CT]) {});
-  } else {
-    staged_loop<T>(oa, ob, K, sA, sB, [&](const uint4* la, const uint4* lb) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        F fa[RT], fb[CT];
-        rd(la, lb, s, fa, fb, 0);
-        rd(la, lb, s, fa, fb, 1);
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
-      }
-    });
-  }
+  pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, rd, [](int, F(&)[RT], F(&)[CT]) {});
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   rows_epilogue<T, MAP, BW, PAIR>(a, acc, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats, group, none,
@@ -107,7 +92,7 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
 // the optional indices. SIDE: the operand whose column sums (the bias gradient) are taken
 // along, by one more product with ones in the tiles at 0 of the other dimension (0 none, 1 A,
 // 2 B).
-template <typename T, bool VEC, int SIDE, typename SH>
+template <typename T, int SIDE, typename SH>
 __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(LinearArgs a) {
   constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
   constexpr Map MAP = out_map<T, false>();
@@ -180,24 +165,7 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
         for (int j = 0; j < CT; ++j) sum[j] = mma(fb[j], ones, sum[j]);
     }
   };
-  if constexpr (VEC) {
-    pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, rd, extra);
-  } else {
-    staged_loop<T>(oa, ob, r1 - r0, sA, sB, [&](const uint4* la, const uint4* lb) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        F fa[RT], fb[CT];
-        rd(la, lb, s, fa, fb, 0);
-        rd(la, lb, s, fa, fb, 1);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-#pragma unroll
-          for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
-          extra(i, fa, fb);
-        }
-      }
-    });
-  }
+  pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, rd, extra);
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats,
@@ -226,43 +194,82 @@ __global__ void __launch_bounds__(256) linear_merge_kernel(const float* part, co
   store_run<4>((is_db ? db : C) + k, s, n);
 }
 
-// dpre = act'(pre) dy over [rows][N]; SwiGLU: pre [rows][2 f], dy [rows][f]. W elements a
-// thread, 16 bytes where the rows allow it.
-template <typename T, int W>
+// dpre = act'(pre) dy over [rows][N]; SwiGLU: pre [rows][2 f], dy [rows][f]. 16 bytes a thread. Rows
+// of dpre are ld elements apart, zeros past the N-th.
+template <typename T>
 __global__ void __launch_bounds__(256) linear_act_grad_kernel(const T* pre, const T* dy, T* dpre,
-                                                              int64_t rows, int f, int act) {
-  const int per = (f + W - 1) / W;
+                                                              int64_t rows, int f, int ld, int act) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int per = (f + W - 1) / W, N = act == PULSAR_ACT_SWIGLU ? 2 * f : f;
   const int64_t total = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * W, n = f - c;
     float g[W], d[W], o[W];
     load_run<W>(dy + r * f + c, d, n);
+    load_run<W>(pre + r * N + c, g, n);
+    T* out = dpre + r * ld;
     if (act == PULSAR_ACT_SWIGLU) {
       float u[W], ou[W];
-      load_run<W>(pre + r * 2 * f + c, g, n);
-      load_run<W>(pre + r * 2 * f + f + c, u, n);
+      load_run<W>(pre + r * N + f + c, u, n);
 #pragma unroll
       for (int q = 0; q < W; ++q) {
         ou[q] = d[q] * g[q] * fast_sigmoid(g[q]);
         o[q] = d[q] * u[q] * act_slope(PULSAR_ACT_SILU, g[q]);
       }
-      store_run<W>(dpre + r * 2 * f + c, o, n);
-      store_run<W>(dpre + r * 2 * f + f + c, ou, n);
+      store_run<W>(out + f + c, ou, n);
     } else {
-      load_run<W>(pre + r * f + c, g, n);
 #pragma unroll
       for (int q = 0; q < W; ++q) o[q] = d[q] * act_slope(act, g[q]);
-      store_run<W>(dpre + r * f + c, o, n);
     }
+    store_run<W>(out + c, o, n);
+    if (n <= W)
+      for (int q = N; q < ld; ++q) out[q] = from_f<T>(0.f);
   }
+}
+
+// Copies of matrices into rows of whole aligned chunks, zeros past their columns: `halves` runs of
+// `cols` columns each, at src_ld per row, to runs of `run` columns. One thread a chunk.
+struct PackJob {
+  const void* src;
+  void* dst;
+  int64_t rows, src_ld, src_group;  // rows of each group
+  int64_t chunks;                   // in all
+  int cols, halves, run;
+};
+struct PackJobs {
+  PackJob job[3];
+};
+template <typename U>
+__global__ void __launch_bounds__(256) linear_pack_kernel(PackJobs jobs) {
+  constexpr int W = 16 / (int)sizeof(U);
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int k = 0;
+  while (k < 3 && i >= jobs.job[k].chunks) i -= jobs.job[k++].chunks;
+  if (k == 3) return;
+  const PackJob& j = jobs.job[k];
+  const int per = j.run / W;
+  const int64_t run = i / per, row = run / j.halves;
+  const int c = (int)(i % per) * W, n = j.cols - c;
+  const U* p = reinterpret_cast<const U*>(j.src) + row / j.rows * j.src_group + row % j.rows * j.src_ld +
+               run % j.halves * j.cols + c;
+  U v[W];
+  if (n >= W) {
+    __builtin_memcpy(v, p, 16);
+  } else {
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[q] = q < n ? p[q] : 0;
+  }
+  uint4 o;
+  __builtin_memcpy(&o, v, 16);
+  reinterpret_cast<uint4*>(j.dst)[i] = o;
 }
 
 typedef LinShape<8, 4, 2, 4, 2> LinWide;   // 256 x 256
 typedef LinShape<4, 4, 2, 2, 2> LinLarge;  // 128 x 128
 typedef LinShape<2, 4, 2, 2, 2> LinSmall;  // 64 x 128
 
-template <typename T, bool BKC, bool PAIR, bool VEC, typename SH>
+template <typename T, bool BKC, bool PAIR, typename SH>
 int launch_rows_shape(LinearArgs& a, hipStream_t s) {
   const int f = PAIR ? a.N / 2 : a.N, obn = PAIR ? SH::BN / 2 : SH::BN;
   // every group adds at most one partial tile to the whole ones
@@ -272,42 +279,60 @@ int launch_rows_shape(LinearArgs& a, hipStream_t s) {
   const int64_t tiles = tiles_r * ((f + obn - 1) / obn);
   a.max_tiles = (int)tiles_r;
   if (tiles > (int64_t)1 << 30) return fail(PULSAR_ERR_INVALID, "linear: launch too large");
-  linear_rows_kernel<T, BKC, PAIR, VEC, SH>
+  linear_rows_kernel<T, BKC, PAIR, SH>
       <<<(unsigned)((tiles + kXcds - 1) / kXcds * kXcds), SH::kThreads, 0, s>>>(a);
   PULSAR_LAUNCH_CHECK();
   return PULSAR_OK;
 }
 
+// Expected us of a product in tiles of BM x BN, by what bounds them here: each CU streams the
+// operands of its tiles from the caches at `rate` bytes/us (35 KB/us for the few-row kernels,
+// 45-49 for the tile kernels with two workgroups a CU, 38 for 256 x 256, whose tiles also pay
+// `each` us of start and end that nothing overlaps) or multiplies at 5 (bf16) or 0.5 (fp32)
+// MFLOP/us, whichever takes longer, after about 4 us of launch and first loads. Measured against
+// it, us (model): 16 rows x 1024 x 1024 in 16 x 16 tiles 5.7 (5.8), in 16 x 32 6.3 (6.7); 512
+// rows 32 x 64 9.7 (9.5), 32 x 32 12.0 (11.3), 64 x 64 12.4 (11.3); 4096 columns x 4096 k, 64
+// rows in 32 x 32 19.7 (18.6), 32 x 64 26 (25.9); 2048 rows in 64 x 128 12.6 (12.5); 16384 x 2048
+// x 1024 in 128 x 128 85 (87), in 256 x 256 77 (79). A ragged launch has about 0.6 partial tiles a
+// group, at least one, and no whole rounds: a quarter of one is added beyond the first.
+double rows_cost(const LinearArgs& a, bool half, int BM, int BN, double rate, double flop_rate,
+                 double each) {
+  double rt = (a.rows + BM - 1) / BM;
+  if (a.offsets)
+    rt = std::max<double>(std::min(a.groups, a.rows), (double)a.rows / BM + 0.6 * a.groups);
+  const double n = rt * ((a.N + BN - 1) / BN) / 256;
+  const double rounds = a.offsets ? (n <= 1 ? 1 : n + 0.25) : std::ceil(n);
+  const double bytes = (double)(BM + BN) * a.K * (half ? 2 : 4), flops = 2.0 * BM * BN * a.K;
+  return 4 + rounds * (each + std::max(bytes / rate, flops / flop_rate));
+}
+
 template <typename T>
 int launch_rows(LinearArgs& a, bool b_kc, hipStream_t s) {
-  const int ev = 16 / (int)sizeof(T);
+  constexpr bool half = sizeof(T) == 2;
   const bool pair = a.act == PULSAR_ACT_SWIGLU;
-  const int f = pair ? a.N / 2 : a.N;
-  const bool vec = aligned16(a.A) && aligned16(a.B) && a.lda % ev == 0 && a.ldb % ev == 0 &&
-                   a.b_group % ev == 0 && a.K % ev == 0 && (b_kc || f % ev == 0);
-  // the launch's tiles, a ragged group adding half of one on average
-  auto tiles = [&](int r, int c) {
-    return ((a.rows + r - 1) / r + (a.offsets ? a.groups / 2 : 0)) * (((int64_t)a.N + c - 1) / c);
+  // the shape that the model expects to be fastest: the few-row ones, then the tiles
+  int best = -1;
+  double least = 0;
+  auto offer = [&](int id, double us) {
+    if (best < 0 || us < least) best = id, least = us;
   };
-  const int64_t t128 = tiles(128, 128), t256 = tiles(256, 256);
-  const double steps = (a.K + 4 * ev * 2 - 1) / (4 * ev * 2);
-  const bool large = t128 >= 256;
-  const bool wide = ((t256 + 255) / 256) * (10 + 1.7 * steps) < ((t128 + 511) / 512) * (5.7 + 0.98 * steps);
-  auto go = [&](auto kc, auto pr, auto vc) {
-    constexpr bool KC = decltype(kc)::value, P = decltype(pr)::value, V = decltype(vc)::value;
-    if constexpr (V && sizeof(T) == 2) {
-      if (wide) return launch_rows_shape<T, KC, P, V, LinWide>(a, s);
+  for (int i = pair ? 1 : 0; i < 6; ++i)
+    offer(i, rows_cost(a, half, 16 * kFewShapes[i].rt, 16 * kFewShapes[i].ct, 35e3,
+                       half ? 5e6 : b_kc ? 0.33e6 : 0.25e6, 0));
+  offer(6, rows_cost(a, half, 64, 128, 45e3, half ? 5e6 : 0.47e6, 0));
+  offer(7, rows_cost(a, half, 128, 128, 49e3, half ? 5e6 : 0.5e6, 0));
+  if (half) offer(8, rows_cost(a, half, 256, 256, 38e3, 5e6, 10));
+  if (best < 6) return launch_linear_few(a, half ? PULSAR_BF16 : PULSAR_F32, b_kc, best, s);
+  auto go = [&](auto kc, auto pr) {
+    constexpr bool KC = decltype(kc)::value, P = decltype(pr)::value;
+    if constexpr (half) {
+      if (best == 8) return launch_rows_shape<T, KC, P, LinWide>(a, s);
     }
-    if (large) return launch_rows_shape<T, KC, P, V, LinLarge>(a, s);
-    return launch_rows_shape<T, KC, P, V, LinSmall>(a, s);
+    return best == 7 ? launch_rows_shape<T, KC, P, LinLarge>(a, s)
+                     : launch_rows_shape<T, KC, P, LinSmall>(a, s);
   };
-  auto pick_vec = [&](auto kc, auto pr) {
-    return vec ? go(kc, pr, std::true_type{}) : go(kc, pr, std::false_type{});
-  };
-  auto pick_pair = [&](auto kc) {
-    return pair ? pick_vec(kc, std::true_type{}) : pick_vec(kc, std::false_type{});
-  };
-  return b_kc ? pick_pair(std::true_type{}) : pick_pair(std::false_type{});
+  if (b_kc) return pair ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  return pair ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 // How a weight gradient is cut: tile shape and splits of the sum over rows. Splits: enough
@@ -330,7 +355,7 @@ WgradPlan wgrad_plan(int64_t rows, int64_t groups, int64_t d_in, int64_t d_out, 
   return {false, tiles(128) >= 384 ? 1 : splits(tiles(128), 512)};
 }
 
-template <typename T, bool VEC, typename SH>
+template <typename T, typename SH>
 int launch_wgrad(LinearArgs& a, int side, hipStream_t s) {
   a.tiles_m = (a.M + SH::BM - 1) / SH::BM;
   a.tiles_n = (a.N + SH::BN - 1) / SH::BN;
@@ -339,11 +364,11 @@ int launch_wgrad(LinearArgs& a, int side, hipStream_t s) {
   const int64_t run = kXcds * std::max<int64_t>(1, per / kXcds);  // place_wgrad's
   const unsigned grid = (unsigned)((tiles + run - 1) / run * run);
   if (side == 0)
-    linear_wgrad_kernel<T, VEC, 0, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    linear_wgrad_kernel<T, 0, SH><<<grid, SH::kThreads, 0, s>>>(a);
   else if (side == 1)
-    linear_wgrad_kernel<T, VEC, 1, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    linear_wgrad_kernel<T, 1, SH><<<grid, SH::kThreads, 0, s>>>(a);
   else
-    linear_wgrad_kernel<T, VEC, 2, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    linear_wgrad_kernel<T, 2, SH><<<grid, SH::kThreads, 0, s>>>(a);
   PULSAR_LAUNCH_CHECK();
   if (a.splits > 1) {
     const int64_t n_c = (int64_t)a.groups * a.M * a.N;
@@ -385,133 +410,220 @@ int check_common(int64_t rows, int64_t groups, int64_t d_in, int64_t d_out, cons
 // Whether the weight is stored with its input dimension contiguous.
 bool in_contiguous(const Weight& w) { return w.in == 1; }
 
-int forward(const void* x, int64_t x_rs, int64_t x_rows, const int32_t* index, const Weight& w,
-            const void* bias, int bias_dtype, const void* residual, int64_t res_rs, void* y,
-            void* pre, const int32_t* offsets, int64_t groups, int64_t rows, int64_t d_in,
-            int64_t d_out, int act, int dtype, hipStream_t s) {
-  if (rows == 0) return PULSAR_OK;
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// A stored matrix: groups of rows, a row contiguous.
+struct Matrix {
+  const void* p;
+  int64_t ld, group, groups, rows, cols;
+  int halves = 1;  // of the columns
+};
+
+// Workspace handed out in 256-byte steps; with base == nullptr it only counts.
+struct Space {
+  char* base;
+  int64_t used = 0;
+  void* take(int64_t bytes) {
+    void* r = base + used;
+    used += round_up(bytes, 256);
+    return r;
+  }
+};
+
+// The kernels read operands in whole 16-byte chunks; a matrix whose rows do not lie that way (odd
+// widths, slices of wider buffers) is copied first, into rows padded with zeros. The copy costs
+// its bytes twice; reading such rows in place ran at a third of the aligned rate (517 rows x
+// 1023 x 777: 25-31 us).
+struct Packing {
+  PackJobs jobs = {};
+  int n = 0;
+  int es;
+  Space& ws;
+  Packing(int es_, Space& ws_) : es(es_), ws(ws_) {}
+  Matrix operator()(Matrix m) {
+    const int64_t ev = 16 / es, cols = m.cols / m.halves;
+    if (aligned16(m.p) && m.ld % ev == 0 && (m.groups == 1 || m.group % ev == 0) && cols % ev == 0) return m;
+    const int64_t run = round_up(cols, ev);
+    PackJob& j = jobs.job[n++];
+    j.src = m.p; j.rows = m.rows; j.src_ld = m.ld; j.src_group = m.group;
+    j.cols = (int)cols; j.halves = m.halves; j.run = (int)run;
+    m.ld = run * m.halves;
+    m.group = m.rows * m.ld;
+    j.chunks = m.groups * m.group / ev;
+    m.p = j.dst = ws.take(m.groups * m.group * es);
+    return m;
+  }
+  int launch(hipStream_t s) const {
+    int64_t chunks = 0;
+    for (int i = 0; i < n; ++i) chunks += jobs.job[i].chunks;
+    if (chunks == 0) return PULSAR_OK;
+    if (chunks > (int64_t)1 << 38) return fail(PULSAR_ERR_INVALID, "linear: operands too large");
+    if (es == 2)
+      linear_pack_kernel<uint16_t><<<blocks_for(chunks, 256), 256, 0, s>>>(jobs);
+    else
+      linear_pack_kernel<uint32_t><<<blocks_for(chunks, 256), 256, 0, s>>>(jobs);
+    PULSAR_LAUNCH_CHECK();
+    return PULSAR_OK;
+  }
+};
+
+// One call's operands, as the C entries take them.
+struct Call {
+  const void* x;
+  int64_t x_rs, x_rows;
+  const int32_t* index;
+  const int32_t* offsets;
+  Weight w;
+  int64_t rows, groups, d_in, d_out;
+  int act, dtype;
+  const char* what;
+
+  int es() const { return dtype == PULSAR_BF16 ? 2 : 4; }
+  Matrix x_matrix() const { return {x, x_rs, 0, 1, x_rows, d_in}; }
+  Matrix w_matrix(bool pair) const {
+    if (in_contiguous(w)) return {w.p, w.out, w.group, groups, d_out, d_in};
+    return {w.p, w.in, w.group, groups, d_in, d_out, pair ? 2 : 1};
+  }
+  int check() const {
+    const int rc = check_common(rows, groups, d_in, d_out, w, act, dtype, what);
+    if (rc != PULSAR_OK) return rc;
+    if (x_rows < 0 || (rows > 0 && x_rs < d_in && x_rows > 1))
+      return fail(PULSAR_ERR_INVALID, std::string(what) + ": rows of x overlap");
+    return PULSAR_OK;
+  }
+  int null_pointer() const { return fail(PULSAR_ERR_INVALID, std::string(what) + ": null pointer"); }
+  int no_workspace() const {
+    return fail(PULSAR_ERR_INVALID, std::string(what) + ": workspace missing or not 16-byte aligned");
+  }
+};
+
+// The operands of a forward call as its kernel takes them, and the workspace they need.
+struct ForwardPlan {
+  Space ws;
+  Packing pack;
+  Matrix x, w;
+  ForwardPlan(const Call& c, void* workspace)
+      : ws{static_cast<char*>(workspace)}, pack(c.es(), ws), x(pack(c.x_matrix())),
+        w(pack(c.w_matrix(c.act == PULSAR_ACT_SWIGLU))) {}
+};
+
+int forward(const Call& c, const void* bias, int bias_dtype, const void* residual, int64_t res_rs,
+            void* y, void* pre, void* workspace, hipStream_t s) {
+  const int rc = c.check();
+  if (rc != PULSAR_OK) return rc;
+  if (bias && bias_dtype != PULSAR_F32 && bias_dtype != PULSAR_BF16)
+    return fail(PULSAR_ERR_INVALID, std::string(c.what) + ": bias dtype must be PULSAR_F32 or PULSAR_BF16");
+  if (c.rows == 0) return PULSAR_OK;
+  if (!y || (!c.x && c.x_rows > 0) || !c.w.p) return c.null_pointer();
+  ForwardPlan plan(c, workspace);
+  if (plan.ws.used > 0 && (!workspace || !aligned16(workspace))) return c.no_workspace();
+  const int rp = plan.pack.launch(s);
+  if (rp != PULSAR_OK) return rp;
+  const bool kc = in_contiguous(c.w), pair = c.act == PULSAR_ACT_SWIGLU;
+  const int64_t f = pair ? c.d_out / 2 : c.d_out;
   LinearArgs a = {};
-  const bool kc = in_contiguous(w);
-  a.A = x; a.lda = x_rs; a.a_rows = index; a.a_nrows = x_rows;
-  a.B = w.p; a.ldb = kc ? w.out : w.in; a.b_group = w.group;
-  a.offsets = offsets; a.groups = (int)groups; a.rows = (int)rows;
-  a.N = (int)d_out; a.K = (int)d_in;
-  a.C = y; a.ldc = act == PULSAR_ACT_SWIGLU ? d_out / 2 : d_out;
-  a.pre = pre; a.ldpre = d_out;
+  a.A = plan.x.p; a.lda = plan.x.ld; a.a_rows = c.index; a.a_nrows = c.x_rows;
+  a.B = plan.w.p; a.ldb = plan.w.ld; a.b_group = plan.w.group;
+  a.up = (int)(kc || plan.w.p == c.w.p ? f : plan.w.ld / 2);
+  a.offsets = c.offsets; a.groups = (int)c.groups; a.rows = (int)c.rows;
+  a.N = (int)c.d_out; a.K = (int)c.d_in;
+  a.C = y; a.ldc = f;
+  a.pre = pre; a.ldpre = c.d_out;
   a.bias = bias; a.bias_dtype = bias_dtype;
   a.residual = residual; a.ldr = res_rs;
-  a.act = act;
-  return dtype == PULSAR_BF16 ? launch_rows<bf16>(a, kc, s) : launch_rows<float>(a, kc, s);
+  a.act = c.act;
+  return c.dtype == PULSAR_BF16 ? launch_rows<bf16>(a, kc, s) : launch_rows<float>(a, kc, s);
 }
 
-int64_t workspace_bytes(int64_t rows, int64_t groups, int64_t d_in, int64_t d_out, int act,
-                        int dtype) {
-  if (rows < 0 || groups < 1 || d_in < 1 || d_out < 1) return -1;
-  const int64_t es = dtype == PULSAR_BF16 ? 2 : 4;
-  const int64_t dpre = act == PULSAR_ACT_NONE ? 0 : (rows * d_out * es + 255) / 256 * 256;
-  const int splits = wgrad_plan(rows, groups, d_in, d_out, dtype).splits;
-  const int64_t part = splits > 1 ? splits * groups * (d_in * d_out + d_out) * 4 : 0;
-  return dpre + part;
-}
+struct BackwardPlan {
+  Space ws;
+  Packing pack;
+  Matrix x, w, dpre;
+  WgradPlan wgrad;
+  float *part = nullptr, *part_db = nullptr;
+  BackwardPlan(const Call& c, const void* dy, void* workspace)
+      : ws{static_cast<char*>(workspace)}, pack(c.es(), ws), x(pack(c.x_matrix())),
+        w(pack(c.w_matrix(false))), dpre{dy, c.d_out, 0, 1, c.rows, c.d_out},
+        wgrad(wgrad_plan(c.rows, c.groups, c.d_in, c.d_out, c.dtype)) {
+    if (c.act == PULSAR_ACT_NONE) {
+      dpre = pack(dpre);
+    } else {
+      dpre.ld = round_up(c.d_out, 16 / c.es());
+      dpre.p = ws.take(c.rows * dpre.ld * c.es());
+    }
+    if (wgrad.splits > 1) {
+      part = static_cast<float*>(ws.take(wgrad.splits * c.groups * c.d_in * c.d_out * 4));
+      part_db = static_cast<float*>(ws.take(wgrad.splits * c.groups * c.d_out * 4));
+    }
+  }
+};
 
 template <typename T>
-int backward_t(const void* dy, const void* x, int64_t x_rs, int64_t x_rows, const int32_t* index,
-               const Weight& w, const void* pre, void* dx, void* dw, void* db,
-               const int32_t* offsets, int64_t groups, int64_t rows, int64_t d_in, int64_t d_out,
-               int act, void* workspace, hipStream_t s) {
-  const int ev = 16 / (int)sizeof(T);
-  const void* dpre = dy;
-  char* ws = static_cast<char*>(workspace);
-  if (act != PULSAR_ACT_NONE && rows > 0) {
-    const int f = (int)(act == PULSAR_ACT_SWIGLU ? d_out / 2 : d_out);
-    const int64_t n = rows * ((f + ev - 1) / ev);
-    linear_act_grad_kernel<T, 16 / (int)sizeof(T)>
-        <<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192), 256, 0, s>>>(
-            static_cast<const T*>(pre), static_cast<const T*>(dy), reinterpret_cast<T*>(ws), rows,
-            f, act);
-    PULSAR_LAUNCH_CHECK();
-    dpre = ws;
-    ws += (rows * d_out * (int64_t)sizeof(T) + 255) / 256 * 256;
-  }
-  const bool kc = in_contiguous(w);
-  if (rows > 0) {
-    LinearArgs a = {};
-    a.A = dpre; a.lda = d_out; a.a_nrows = rows;
+int backward_t(const Call& c, const BackwardPlan& plan, const void* dy, const void* pre, void* dx,
+               void* dw, void* db, hipStream_t s) {
+  const bool kc = in_contiguous(c.w);
+  if (c.rows > 0) {
+    const int rp = plan.pack.launch(s);
+    if (rp != PULSAR_OK) return rp;
+    if (c.act != PULSAR_ACT_NONE) {
+      constexpr int ev = 16 / (int)sizeof(T);
+      const int f = (int)(c.act == PULSAR_ACT_SWIGLU ? c.d_out / 2 : c.d_out);
+      const int64_t n = c.rows * ((f + ev - 1) / ev);
+      linear_act_grad_kernel<T><<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192), 256, 0, s>>>(
+          static_cast<const T*>(pre), static_cast<const T*>(dy),
+          static_cast<T*>(const_cast<void*>(plan.dpre.p)), c.rows, f, (int)plan.dpre.ld, c.act);
+      PULSAR_LAUNCH_CHECK();
+    }
     // dx = dpre w^T: n is the input dimension, k the output one
-    a.B = w.p; a.ldb = kc ? w.out : w.in; a.b_group = w.group;
-    a.offsets = offsets; a.groups = (int)groups; a.rows = (int)rows;
-    a.N = (int)d_in; a.K = (int)d_out;
-    a.C = dx; a.ldc = d_in;
-    a.act = PULSAR_ACT_NONE;
+    LinearArgs a = {};
+    a.A = plan.dpre.p; a.lda = plan.dpre.ld; a.a_nrows = c.rows;
+    a.B = plan.w.p; a.ldb = plan.w.ld; a.b_group = plan.w.group;
+    a.offsets = c.offsets; a.groups = (int)c.groups; a.rows = (int)c.rows;
+    a.N = (int)c.d_in; a.K = (int)c.d_out;
+    a.C = dx; a.ldc = c.d_in;
     const int rc = launch_rows<T>(a, !kc, s);
     if (rc != PULSAR_OK) return rc;
   }
+  // dw in the weight's own order: its contiguous dimension is n
   LinearArgs a = {};
-  // C in the weight's own order: its contiguous dimension is n
-  const bool dpre_a = kc;
-  if (dpre_a) {
-    a.A = dpre; a.lda = d_out; a.a_nrows = rows; a.M = (int)d_out;
-    a.B = x; a.ldb = x_rs; a.b_rows = index; a.b_nrows = x_rows; a.N = (int)d_in;
+  if (kc) {
+    a.A = plan.dpre.p; a.lda = plan.dpre.ld; a.a_nrows = c.rows; a.M = (int)c.d_out;
+    a.B = plan.x.p; a.ldb = plan.x.ld; a.b_rows = c.index; a.b_nrows = c.x_rows; a.N = (int)c.d_in;
   } else {
-    a.A = x; a.lda = x_rs; a.a_rows = index; a.a_nrows = x_rows; a.M = (int)d_in;
-    a.B = dpre; a.ldb = d_out; a.b_nrows = rows; a.N = (int)d_out;
+    a.A = plan.x.p; a.lda = plan.x.ld; a.a_rows = c.index; a.a_nrows = c.x_rows; a.M = (int)c.d_in;
+    a.B = plan.dpre.p; a.ldb = plan.dpre.ld; a.b_nrows = c.rows; a.N = (int)c.d_out;
   }
-  a.offsets = offsets; a.groups = (int)groups; a.rows = (int)rows;
+  a.offsets = c.offsets; a.groups = (int)c.groups; a.rows = (int)c.rows;
   a.C = dw; a.ldc = a.N; a.c_group = (int64_t)a.M * a.N;
   a.db = db;
-  const WgradPlan plan = wgrad_plan(rows, groups, d_in, d_out, sizeof(T) == 2 ? PULSAR_BF16 : PULSAR_F32);
-  a.splits = plan.splits;
-  if (a.splits > 1) {
-    a.part = reinterpret_cast<float*>(ws);
-    a.part_db = a.part + (int64_t)a.splits * groups * d_in * d_out;
-  }
-  const bool vec = aligned16(a.A) && aligned16(a.B) && a.lda % ev == 0 && a.ldb % ev == 0 &&
-                   a.M % ev == 0 && a.N % ev == 0;
-  const int side = db ? (dpre_a ? 1 : 2) : 0;
+  a.splits = plan.wgrad.splits;
+  a.part = plan.part;
+  a.part_db = plan.part_db;
+  const int side = db ? (kc ? 1 : 2) : 0;
   if constexpr (sizeof(T) == 2) {
-    if (plan.wide && vec) return launch_wgrad<T, true, LinWide>(a, side, s);
+    if (plan.wgrad.wide) return launch_wgrad<T, LinWide>(a, side, s);
   }
-  return vec ? launch_wgrad<T, true, LinLarge>(a, side, s) : launch_wgrad<T, false, LinLarge>(a, side, s);
+  return launch_wgrad<T, LinLarge>(a, side, s);
 }
 
-int null_check(const char* what) {
-  return fail(PULSAR_ERR_INVALID, std::string(what) + ": null pointer");
-}
-
-int backward(const void* dy, const void* x, int64_t x_rs, int64_t x_rows, const int32_t* index,
-             const Weight& w, const void* pre, void* dx, void* dw, void* db, const int32_t* offsets,
-             int64_t groups, int64_t rows, int64_t d_in, int64_t d_out, int act, int dtype,
-             void* workspace, hipStream_t s, const char* what) {
-  const int rc = check_common(rows, groups, d_in, d_out, w, act, dtype, what);
+int backward(const Call& c, const void* dy, const void* pre, void* dx, void* dw, void* db,
+             void* workspace, hipStream_t s) {
+  const int rc = c.check();
   if (rc != PULSAR_OK) return rc;
-  if (!dw || (rows > 0 && (!dy || (!x && x_rows > 0) || !w.p || !dx || (act != PULSAR_ACT_NONE && !pre))))
-    return null_check(what);
-  if (rows > 0 && x_rs < d_in && x_rows > 1)
-    return fail(PULSAR_ERR_INVALID, std::string(what) + ": rows of x overlap");
-  if (workspace_bytes(rows, groups, d_in, d_out, act, dtype) > 0 &&
-      (!workspace || !aligned16(workspace)))
-    return fail(PULSAR_ERR_INVALID, std::string(what) + ": workspace missing or not 16-byte aligned");
-  if (dtype == PULSAR_BF16)
-    return backward_t<bf16>(dy, x, x_rs, x_rows, index, w, pre, dx, dw, db, offsets, groups, rows,
-                            d_in, d_out, act, workspace, s);
-  return backward_t<float>(dy, x, x_rs, x_rows, index, w, pre, dx, dw, db, offsets, groups, rows,
-                           d_in, d_out, act, workspace, s);
+  if (!dw || (c.rows > 0 && (!dy || (!c.x && c.x_rows > 0) || !c.w.p || !dx ||
+                             (c.act != PULSAR_ACT_NONE && !pre))))
+    return c.null_pointer();
+  BackwardPlan plan(c, dy, workspace);
+  if (plan.ws.used > 0 && (!workspace || !aligned16(workspace))) return c.no_workspace();
+  return c.dtype == PULSAR_BF16 ? backward_t<bf16>(c, plan, dy, pre, dx, dw, db, s)
+                                : backward_t<float>(c, plan, dy, pre, dx, dw, db, s);
 }
 
-int forward_checked(const void* x, int64_t x_rs, int64_t x_rows, const int32_t* index,
-                    const Weight& w, const void* bias, int bias_dtype, const void* residual,
-                    int64_t res_rs, void* y, void* pre, const int32_t* offsets, int64_t groups,
-                    int64_t rows, int64_t d_in, int64_t d_out, int act, int dtype, hipStream_t s,
-                    const char* what) {
-  const int rc = check_common(rows, groups, d_in, d_out, w, act, dtype, what);
-  if (rc != PULSAR_OK) return rc;
-  if (rows > 0 && (!y || (!x && x_rows > 0) || !w.p)) return null_check(what);
-  if (bias && bias_dtype != PULSAR_F32 && bias_dtype != PULSAR_BF16)
-    return fail(PULSAR_ERR_INVALID, std::string(what) + ": bias dtype must be PULSAR_F32 or PULSAR_BF16");
-  if (rows > 0 && x_rs < d_in && x_rows > 1)
-    return fail(PULSAR_ERR_INVALID, std::string(what) + ": rows of x overlap");
-  return forward(x, x_rs, x_rows, index, w, bias, bias_dtype, residual, res_rs, y, pre, offsets,
-                 groups, rows, d_in, d_out, act, dtype, s);
+int64_t forward_bytes(const Call& c) {
+  return c.check() != PULSAR_OK ? -1 : c.rows == 0 ? 0 : ForwardPlan(c, nullptr).ws.used;
+}
+int64_t backward_bytes(const Call& c, const void* dy) {
+  return c.check() != PULSAR_OK ? -1 : BackwardPlan(c, dy, nullptr).ws.used;
 }
 
 }  // namespace
@@ -522,28 +634,48 @@ using namespace pulsar;
 
 extern "C" {
 
+int64_t pulsar_fused_linear_forward_workspace_bytes(const void* x, int64_t x_rs, const void* w,
+                                                    int64_t w_out, int64_t w_in, int64_t rows,
+                                                    int64_t d_in, int64_t d_out, int activation,
+                                                    int dtype) {
+  return forward_bytes(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
+                            d_out, activation, dtype, "fused_linear_forward"});
+}
+
 int pulsar_fused_linear_forward(const void* x, int64_t x_rs, const void* w, int64_t w_out,
                                 int64_t w_in, const void* bias, int bias_dtype,
                                 const void* residual, int64_t residual_rs, void* y, void* pre,
                                 int64_t rows, int64_t d_in, int64_t d_out, int activation,
-                                int dtype, hipStream_t stream) {
-  return forward_checked(x, x_rs, rows, nullptr, Weight{w, 0, w_in, w_out}, bias, bias_dtype,
-                         residual, residual_rs, y, pre, nullptr, 1, rows, d_in, d_out, activation,
-                         dtype, stream, "fused_linear_forward");
+                                int dtype, void* workspace, hipStream_t stream) {
+  return forward(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in, d_out,
+                      activation, dtype, "fused_linear_forward"},
+                 bias, bias_dtype, residual, residual_rs, y, pre, workspace, stream);
 }
 
-int64_t pulsar_fused_linear_backward_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out,
+int64_t pulsar_fused_linear_backward_workspace_bytes(const void* dy, const void* x, int64_t x_rs,
+                                                     const void* w, int64_t w_out, int64_t w_in,
+                                                     int64_t rows, int64_t d_in, int64_t d_out,
                                                      int activation, int dtype) {
-  return workspace_bytes(rows, 1, d_in, d_out, activation, dtype);
+  return backward_bytes(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
+                             d_out, activation, dtype, "fused_linear_backward"}, dy);
 }
 
 int pulsar_fused_linear_backward(const void* dy, const void* x, int64_t x_rs, const void* w,
                                  int64_t w_out, int64_t w_in, const void* pre, void* dx, void* dw,
                                  void* db, int64_t rows, int64_t d_in, int64_t d_out,
                                  int activation, int dtype, void* workspace, hipStream_t stream) {
-  return backward(dy, x, x_rs, rows, nullptr, Weight{w, 0, w_in, w_out}, pre, dx, dw, db, nullptr,
-                  1, rows, d_in, d_out, activation, dtype, workspace, stream,
-                  "fused_linear_backward");
+  return backward(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
+                       d_out, activation, dtype, "fused_linear_backward"},
+                  dy, pre, dx, dw, db, workspace, stream);
+}
+
+int64_t pulsar_grouped_linear_forward_workspace_bytes(const void* x, int64_t x_rs, int64_t x_rows,
+                                                      const void* w, int64_t w_group, int64_t w_in,
+                                                      int64_t w_out, int64_t rows, int64_t groups,
+                                                      int64_t d_in, int64_t d_out, int activation,
+                                                      int dtype) {
+  return forward_bytes(Call{x, x_rs, x_rows, nullptr, nullptr, Weight{w, w_group, w_in, w_out}, rows,
+                            groups, d_in, d_out, activation, dtype, "grouped_linear_forward"});
 }
 
 int pulsar_grouped_linear_forward(const void* x, int64_t x_rs, int64_t x_rows,
@@ -551,16 +683,20 @@ int pulsar_grouped_linear_forward(const void* x, int64_t x_rs, int64_t x_rows,
                                   int64_t w_group, int64_t w_in, int64_t w_out, const void* bias,
                                   int bias_dtype, void* y, void* pre, int64_t rows,
                                   int64_t groups, int64_t d_in, int64_t d_out, int activation,
-                                  int dtype, hipStream_t stream) {
+                                  int dtype, void* workspace, hipStream_t stream) {
   PULSAR_REQUIRE(offsets, "grouped_linear_forward: null pointer");
-  return forward_checked(x, x_rs, x_rows, row_index, Weight{w, w_group, w_in, w_out}, bias,
-                         bias_dtype, nullptr, 0, y, pre, offsets, groups, rows, d_in, d_out,
-                         activation, dtype, stream, "grouped_linear_forward");
+  return forward(Call{x, x_rs, x_rows, row_index, offsets, Weight{w, w_group, w_in, w_out}, rows,
+                      groups, d_in, d_out, activation, dtype, "grouped_linear_forward"},
+                 bias, bias_dtype, nullptr, 0, y, pre, workspace, stream);
 }
 
-int64_t pulsar_grouped_linear_backward_workspace_bytes(int64_t rows, int64_t groups, int64_t d_in,
+int64_t pulsar_grouped_linear_backward_workspace_bytes(const void* dy, const void* x, int64_t x_rs,
+                                                       int64_t x_rows, const void* w,
+                                                       int64_t w_group, int64_t w_in, int64_t w_out,
+                                                       int64_t rows, int64_t groups, int64_t d_in,
                                                        int64_t d_out, int activation, int dtype) {
-  return workspace_bytes(rows, groups, d_in, d_out, activation, dtype);
+  return backward_bytes(Call{x, x_rs, x_rows, nullptr, nullptr, Weight{w, w_group, w_in, w_out}, rows,
+                             groups, d_in, d_out, activation, dtype, "grouped_linear_backward"}, dy);
 }
 
 int pulsar_grouped_linear_backward(const void* dy, const void* x, int64_t x_rs, int64_t x_rows,
@@ -570,9 +706,9 @@ int pulsar_grouped_linear_backward(const void* dy, const void* x, int64_t x_rs, 
                                    int64_t d_in, int64_t d_out, int activation, int dtype,
                                    void* workspace, hipStream_t stream) {
   PULSAR_REQUIRE(offsets, "grouped_linear_backward: null pointer");
-  return backward(dy, x, x_rs, x_rows, row_index, Weight{w, w_group, w_in, w_out}, pre, dx, dw, db,
-                  offsets, groups, rows, d_in, d_out, activation, dtype, workspace, stream,
-                  "grouped_linear_backward");
+  return backward(Call{x, x_rs, x_rows, row_index, offsets, Weight{w, w_group, w_in, w_out}, rows,
+                       groups, d_in, d_out, activation, dtype, "grouped_linear_backward"},
+                  dy, pre, dx, dw, db, workspace, stream);
 }
 
 }  // extern "C"

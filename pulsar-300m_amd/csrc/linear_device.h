@@ -47,7 +47,8 @@ struct LinShape {
 //   BLOCK (fp32, k strided): B = 4 or 2 tiles share each LDS read, 16 B (t / B) + B i + t % B.
 enum Map { PLAIN, WIDE, BLOCK };
 
-// Stages one operand's tile of R rows x 128 bytes of k (64 bf16 or 32 fp32) in LDS.
+// Stages one operand's tile of R rows x 128 bytes of k (64 bf16 or 32 fp32) in LDS. Operands
+// come in whole chunks of 16 bytes, aligned (others are copied so first).
 //   KC (k contiguous in memory): LDS [R][8] chunks of 16 bytes; chunk c of row r sits at
 //     c ^ key(r), which spreads the 16 rows a fragment read takes over the banks.
 //   otherwise (rows of R contiguous elements per k): LDS [k][R]. bf16 tiles are read through
@@ -66,7 +67,7 @@ struct Operand {
   int64_t k_nrows;
   uint32_t ok;            // KC: rows that exist
   int off;                // KC: first k of this thread's chunks; else: its first k row
-  int valid;              // !KC: elements of this thread's chunk columns inside the matrix
+  bool valid;             // !KC: this thread's chunk columns lie inside the matrix
   int index;              // !KC with k_rows: the lane's row of the step to be loaded next
 
   __device__ __forceinline__ static int key(int r) {
@@ -95,8 +96,8 @@ struct Operand {
     if constexpr (sizeof(T) == 2) lc = (((c >> 1) ^ (off & 3)) << 1) | (c & 1);
     int lim;
     const int g = col(lc * EV, lim);
-    valid = min(max(lim - g, 0), EV);
-    base[0] = p + (valid > 0 ? g : 0);
+    valid = g < lim;
+    base[0] = p + (valid ? g : 0);
     ld = ld_;
     k_rows = rows;
     k_nrows = nrows;
@@ -110,56 +111,26 @@ struct Operand {
       index = k < K ? k_rows[k] : -1;
     }
   }
-  // Address and number of elements of chunk i at k step k0 of a matrix with K k's.
-  __device__ __forceinline__ const T* chunk(int i, int k0, int K, int& n) const {
+  // Loads chunk i of k step k0 of a matrix with K k's, zeros for what it does not have.
+  __device__ __forceinline__ void fetch(int i, int k0, int K, uint32_t lds) const {
+    const T* p;
+    bool in;
     if constexpr (KC) {
       const int k = k0 + off;
-      n = (ok >> i & 1) ? min(max(K - k, 0), EV) : 0;
-      return base[i] + k;
+      in = (ok >> i & 1) && k < K;
+      p = base[i] + k;
     } else {
       const int k = k0 + off + i * (THREADS * EV / R);
-      n = k < K ? valid : 0;
+      in = valid && k < K;
       int64_t r = k;
       if (k_rows) {
         r = __shfl(index, off + i * (THREADS * EV / R), 64);
-        if (r < 0 || r >= k_nrows) n = 0;
+        in = in && r >= 0 && r < k_nrows;
       }
-      return base[0] + r * ld;
+      p = base[0] + r * ld;
     }
-  }
-  // Direct load of chunk i: 16-byte aligned, whole or absent.
-  __device__ __forceinline__ void fetch(int i, int k0, int K, uint32_t lds) const {
     const uint32_t w = __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63);
-    int n;
-    const T* p = chunk(i, k0, K, n);
-    load_lds16_at(n > 0 ? (const void*)p : (const void*)&kZeroChunk, lds + (w + i * THREADS) * 16);
-  }
-  // Any alignment: through registers, the partial chunk of a row's end element by element.
-  __device__ __forceinline__ void load(int k0, int K, uint4 (&r)[NCH]) const {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      int n;
-      const T* p = chunk(i, k0, K, n);
-      r[i] = uint4{0u, 0u, 0u, 0u};
-      if (n == EV) {
-        __builtin_memcpy(&r[i], p, 16);
-      } else if (n > 0) {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int e = 0; e < EV; ++e) {
-          if (e >= n) continue;
-          if constexpr (sizeof(T) == 2)
-            w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
-          else
-            w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-        }
-        r[i] = uint4{w[0], w[1], w[2], w[3]};
-      }
-    }
-  }
-  __device__ __forceinline__ void store(const uint4 (&r)[NCH], uint4* lds) const {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) lds[threadIdx.x + i * THREADS] = r[i];
+    load_lds16_at(in ? (const void*)p : (const void*)&kZeroChunk, lds + (w + i * THREADS) * 16);
   }
 };
 
@@ -318,38 +289,6 @@ __device__ __forceinline__ void pipe_loop(OA& oa, OB& ob, int K, uint4* sA, uint
   wait_vmcnt<0>();  // the loads past the end: their buffers are used again
 }
 
-// The main loop for operands of any alignment: through registers, two LDS buffers.
-template <typename T, typename OA, typename OB, typename F>
-__device__ __forceinline__ void staged_loop(OA& oa, OB& ob, int K, uint4* sA, uint4* sB,
-                                            F&& compute) {
-  constexpr int BK = OA::BK;
-  const int steps = (K + BK - 1) / BK;
-  if (steps == 0) return;
-  uint4 ra[OA::NCH], rb[OB::NCH];
-  auto load = [&](int k0) {
-    oa.load(k0, K, ra);
-    ob.load(k0, K, rb);
-    oa.prefetch(k0 + BK, K);
-    ob.prefetch(k0 + BK, K);
-  };
-  oa.prefetch(0, K);
-  ob.prefetch(0, K);
-  load(0);
-  oa.store(ra, sA);
-  ob.store(rb, sB);
-  __syncthreads();
-  for (int kt = 0; kt < steps; ++kt) {
-    const int b = kt & 1;
-    if (kt + 1 < steps) load((kt + 1) * BK);
-    compute(sA + b * OA::kChunks, sB + b * OB::kChunks);
-    if (kt + 1 < steps) {
-      oa.store(ra, sA + (b ^ 1) * OA::kChunks);
-      ob.store(rb, sB + (b ^ 1) * OB::kChunks);
-    }
-    __syncthreads();
-  }
-}
-
 // Rows [r0, r1) of group g, kept inside the matrix whatever the offsets hold; group `groups` is
 // the rows past the last one.
 __device__ __forceinline__ void group_span(const LinearArgs& a, int g, int& r0, int& r1) {
@@ -428,6 +367,33 @@ __device__ __forceinline__ bool place_tile(int tiles_r, int tiles_c, int& tr, in
   if (slot >= per || item >= total) return false;
   band_tile(item, kBand, tiles_r, tiles_c, tr, tc);
   return true;
+}
+
+// The tile of this workgroup: column block tc, rows r0 .. of group `group`, whose end is r1.
+template <int BM>
+__device__ __forceinline__ bool locate_tile(const LinearArgs& a, int tiles_c, int& tc, int& group,
+                                            int& r0, int& r1) {
+  int tr;
+  if (a.groups < 64) {  // one look at the offsets (their loads are the start of every chain here)
+    const int lane = (int)threadIdx.x & 63;
+    int s0 = 0, s1 = 0;
+    if (lane <= a.groups) group_span(a, lane, s0, s1);
+    const int nt = s1 > s0 ? (s1 - s0 + BM - 1) / BM : 0;
+    int incl = nt;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += v;
+    }
+    const int tiles_r = min(__builtin_amdgcn_readlane(incl, 63), a.max_tiles);
+    if (!place_tile(tiles_r, tiles_c, tr, tc)) return false;
+    group = (int)__builtin_popcountll(__ballot(incl <= tr));
+    r1 = __builtin_amdgcn_readlane(s1, group);
+    r0 = __builtin_amdgcn_readlane(s0, group) +
+         (tr - __builtin_amdgcn_readlane(incl - nt, group)) * BM;
+    return true;
+  }
+  return place_tile(count_tiles<BM>(a), tiles_c, tr, tc) && find_tile<BM>(a, tr, group, r0, r1);
 }
 
 // Weight-gradient tiles: group by group, the largest groups first (up to 64 groups), so that the
@@ -511,36 +477,82 @@ struct Slab {
   static constexpr int kCols = 16 * CT, kStride = kCols + 4, kFloats = 32 * kStride;
 };
 
-// Writes row tiles i, i + 1 of the accumulators: LDS row 16 t + i16, columns in order.
-template <Map MAP, int BW, int NCT, int RT, int CT>
-__device__ __forceinline__ void slab_write(float* slab, const lin_f32x4 (&acc)[RT][CT], int i) {
+// Writes one row tile of accumulators: LDS row i16, columns in order.
+template <Map MAP, int BW, int NCT, int CT>
+__device__ __forceinline__ void slab_write_tile(float* slab, const lin_f32x4 (&acc)[CT]) {
   const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
-  float* l = slab + i16 * Slab<CT>::kStride;
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int j = 0; j < CT; ++j) {
+    // tiles beyond NCT are the second set of a pair, 16 NCT columns on
+    const int u = j % NCT;
+    float* p = slab + i16 * Slab<CT>::kStride + j / NCT * 16 * NCT;
+    if constexpr (MAP == BLOCK) {
+      // element e of tile u: column 16 BW (u / BW) + BW (4 kq + e) + u % BW
+      if (u % BW) continue;
 #pragma unroll
-    for (int j = 0; j < CT; ++j) {
-      // tiles beyond NCT are the second set of a pair, 16 NCT columns on
-      const int set = j / NCT, u = j % NCT;
-      float* p = l + t * 16 * Slab<CT>::kStride + set * 16 * NCT;
-      if constexpr (MAP == BLOCK) {
-        // element e of tile u: column 16 BW (u / BW) + BW (4 kq + e) + u % BW
-        if (u % BW) continue;
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int b = 0; b < BW; ++b)
-            p[16 * u + BW * (4 * kq + e) + b] = acc[i + t][j + b][e];
-      } else {
-        // 4 consecutive columns of element rows 4 kq ..
-        *reinterpret_cast<lin_f32x4*>(p + map_row<MAP, BW>(u, 0) + (MAP == WIDE ? 8 : 4) * kq) =
-            acc[i + t][j];
-      }
+        for (int b = 0; b < BW; ++b) p[16 * u + BW * (4 * kq + e) + b] = acc[j + b][e];
+    } else {
+      // 4 consecutive columns
+      *reinterpret_cast<lin_f32x4*>(p + map_row<MAP, BW>(u, 0) + (MAP == WIDE ? 8 : 4) * kq) = acc[j];
     }
+  }
 }
 
-// Epilogue of a product's tile: bias, activation and residual in fp32, one rounding per output.
-// The wave's accumulators start at row r0 and output column c0; of `f` output columns and rows
+// The bias of 8 columns, of both halves for a pair.
+template <bool PAIR>
+__device__ __forceinline__ void load_bias(const LinearArgs& a, int group, bool none, int col, int f,
+                                          float (&bias)[2][8]) {
+  const int n = f - col;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) bias[h][q] = 0.f;
+  if (!a.bias || none || n <= 0) return;
+#pragma unroll
+  for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
+    const int64_t o = (int64_t)group * a.N + col + h * f;
+    if (a.bias_dtype == PULSAR_F32)
+      load_run<8>(reinterpret_cast<const float*>(a.bias) + o, bias[h], n);
+    else
+      load_run<8>(reinterpret_cast<const bf16*>(a.bias) + o, bias[h], n);
+  }
+}
+
+// 8 columns of row r from their sums v (and u, a pair's second half): bias, activation and
+// residual in fp32, one rounding per output.
+template <typename T, bool PAIR>
+__device__ __forceinline__ void finish_run(const LinearArgs& a, int act, int64_t r, int col, int f,
+                                           float (&v)[8], float (&u)[8], const float (&bias)[2][8]) {
+  const int n = f - col;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    v[q] += bias[0][q];
+    if constexpr (PAIR) u[q] += bias[1][q];
+  }
+  if (a.pre) {
+    T* pre = reinterpret_cast<T*>(a.pre) + r * a.ldpre + col;
+    store_run<8>(pre, v, n);
+    if constexpr (PAIR) store_run<8>(pre + f, u, n);
+  }
+  if constexpr (PAIR) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = v[q] * fast_sigmoid(v[q]) * u[q];
+  } else if (act != PULSAR_ACT_NONE) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = act_value(act, v[q]);
+  }
+  if (a.residual) {
+    float x[8];
+    load_run<8>(reinterpret_cast<const T*>(a.residual) + r * a.ldr + col, x, n);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] += x[q];
+  }
+  store_run<8>(reinterpret_cast<T*>(a.C) + r * a.ldc + col, v, n);
+}
+
+// Epilogue of a product's tile. The wave's accumulators start at row r0 and output column c0; of `f` output columns and rows
 // below r1 only those inside are stored. PAIR: the second half of the CT tiles are the
 // up-projection twins of the first.
 template <typename T, Map MAP, int BW, bool PAIR, int RT, int CT>
@@ -551,24 +563,13 @@ __device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&a
   static_assert(64 % LPR == 0, "whole rows per pass");
   const int lane = (int)threadIdx.x & 63, lc = (lane % LPR) * 8, lr = lane / LPR;
   const int col = c0 + lc, n = f - col;
-  float bias[2][8] = {};
-  if (a.bias && !none && n > 0) {
-#pragma unroll
-    for (int h = 0; h < (PAIR ? 2 : 1); ++h) {
-      const int64_t o = (int64_t)group * a.N + col + h * f;
-      if (a.bias_dtype == PULSAR_F32)
-        load_run<8>(reinterpret_cast<const float*>(a.bias) + o, bias[h], n);
-      else
-        load_run<8>(reinterpret_cast<const bf16*>(a.bias) + o, bias[h], n);
-    }
-  }
-  T* C = reinterpret_cast<T*>(a.C);
-  T* pre = reinterpret_cast<T*>(a.pre);
-  const T* res = reinterpret_cast<const T*>(a.residual);
+  float bias[2][8];
+  load_bias<PAIR>(a, group, none, col, f, bias);
   const int act = none ? PULSAR_ACT_NONE : a.act;
 #pragma unroll
   for (int i = 0; i < RT; i += 2) {
-    slab_write<MAP, BW, NCT>(slab, acc, i);
+    slab_write_tile<MAP, BW, NCT>(slab, acc[i]);
+    slab_write_tile<MAP, BW, NCT>(slab + 16 * Slab<CT>::kStride, acc[i + 1]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 1
     for (int p = lr; p < 32; p += RPI) {
@@ -577,29 +578,11 @@ __device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&a
       float v[8], u[8];
       const float* l = slab + p * Slab<CT>::kStride + lc;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = l[q] + bias[0][q];
-      if constexpr (PAIR) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) u[q] = l[16 * NCT + q] + bias[1][q];
+      for (int q = 0; q < 8; ++q) {
+        v[q] = l[q];
+        u[q] = PAIR ? l[16 * NCT + q] : 0.f;
       }
-      if (pre) {
-        store_run<8>(pre + r * a.ldpre + col, v, n);
-        if constexpr (PAIR) store_run<8>(pre + r * a.ldpre + f + col, u, n);
-      }
-      if constexpr (PAIR) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = v[q] * fast_sigmoid(v[q]) * u[q];
-      } else if (act != PULSAR_ACT_NONE) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = act_value(act, v[q]);
-      }
-      if (res) {
-        float x[8];
-        load_run<8>(res + r * a.ldr + col, x, n);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] += x[q];
-      }
-      store_run<8>(C + r * a.ldc + col, v, n);
+      finish_run<T, PAIR>(a, act, r, col, f, v, u, bias);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next rows overwrite
   }
@@ -617,7 +600,8 @@ __device__ __forceinline__ void wgrad_epilogue(const LinearArgs& a, lin_f32x4 (&
   const int64_t pg = (int64_t)split * a.groups + group;  // a split's partial results
 #pragma unroll
   for (int i = 0; i < RT; i += 2) {
-    slab_write<MAP, BWC, CT>(slab, acc, i);
+    slab_write_tile<MAP, BWC, CT>(slab, acc[i]);
+    slab_write_tile<MAP, BWC, CT>(slab + 16 * Slab<CT>::kStride, acc[i + 1]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 1
     for (int p = lr; p < 32; p += RPI) {

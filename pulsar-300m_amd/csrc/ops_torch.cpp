@@ -361,6 +361,13 @@ PyObject* triple(const Tensor& a, const Tensor& b, const Tensor& c, bool list) {
   return r;
 }
 
+// Workspace of the given size (an error for -1: what the library refuses), undefined when none.
+Tensor workspace(const Tensor& on, int64_t bytes) {
+  if (bytes < 0) throw std::runtime_error(pulsar_last_error());
+  return bytes ? make(on, {bytes}, at::kByte) : Tensor();
+}
+void* wp(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
 // (topk_idx, E) -> (offsets, rows, slots)
 PyObject* moe_group_rows(const Args& a) {
   const Tensor& idx = a.t(0);
@@ -371,7 +378,7 @@ PyObject* moe_group_rows(const Args& a) {
   Tensor s = make(idx, {N, K}, at::kInt), ws;
   if (bytes > 0) ws = make(idx, {bytes / 4}, at::kInt);
   run(pulsar_moe_group_rows, p<int64_t>(idx), q<int32_t>(o), q<int32_t>(r), q<int32_t>(s), N, K, E,
-      const_cast<void*>(p(ws)), stream(idx));
+      wp(ws), stream(idx));
   return triple(o, r, s, false);
 }
 
@@ -390,8 +397,11 @@ PyObject* fused_linear_forward(const Args& a) {
   if (a.i64(5)) pre = make(x, shape);
   if (act == PULSAR_ACT_SWIGLU) shape.back() = O / 2;
   Tensor y = make(x, shape);
+  const Tensor ws = workspace(x, pulsar_fused_linear_forward_workspace_bytes(
+      x.data_ptr(), xs, w.data_ptr(), so, si, rows, I, O, (int)act, code(x)));
   run(pulsar_fused_linear_forward, p(x), xs, p(w), so, si, p(b), b.defined() ? code(b) : 0, p(res),
-      rs, q(y), pre.defined() ? q(pre) : nullptr, rows, I, O, (int)act, code(x), stream(x));
+      rs, q(y), pre.defined() ? q(pre) : nullptr, rows, I, O, (int)act, code(x), wp(ws),
+      stream(x));
   return pre.defined() ? pair(y, pre, false) : out(y);
 }
 
@@ -404,13 +414,12 @@ PyObject* fused_linear_backward(const Args& a) {
   weight_strides(w, so, si);
   const int64_t xs = row_stride(x, "x");
   const c10::DeviceGuard guard(x.device());
-  Tensor dx = make(x, x.sizes()), dw = weight_grad(w, si == 1), db, ws;
+  Tensor dx = make(x, x.sizes()), dw = weight_grad(w, si == 1), db;
   if (a.i64(5)) db = make(x, {O});
-  const int64_t bytes = pulsar_fused_linear_backward_workspace_bytes(rows, I, O, (int)act, code(x));
-  if (bytes > 0) ws = make(x, {bytes}, at::kByte);
+  const Tensor ws = workspace(x, pulsar_fused_linear_backward_workspace_bytes(
+      dy.data_ptr(), x.data_ptr(), xs, w.data_ptr(), so, si, rows, I, O, (int)act, code(x)));
   run(pulsar_fused_linear_backward, p(dy), p(x), xs, p(w), so, si, p(pre), q(dx), q(dw),
-      db.defined() ? q(db) : nullptr, rows, I, O, (int)act, code(x), const_cast<void*>(p(ws)),
-      stream(x));
+      db.defined() ? q(db) : nullptr, rows, I, O, (int)act, code(x), wp(ws), stream(x));
   return triple(dx, dw, db, true);
 }
 
@@ -427,9 +436,12 @@ PyObject* grouped_linear_forward(const Args& a) {
   Tensor pre;
   if (a.i64(6)) pre = make(x, {M, O});
   Tensor y = make(x, {M, act == PULSAR_ACT_SWIGLU ? O / 2 : O});
+  const Tensor ws = workspace(x, pulsar_grouped_linear_forward_workspace_bytes(
+      x.data_ptr(), xs, x.size(0), w.data_ptr(), w.stride(0), si, so, M, E, I, O, (int)act, code(x)));
   run(pulsar_grouped_linear_forward, p(x), xs, x.size(0), p<int32_t>(idx), p<int32_t>(off), p(w),
       w.stride(0), si, so, p(b), b.defined() ? code(b) : 0, q(y),
-      pre.defined() ? q(pre) : nullptr, M, E, I, O, (int)act, code(x), stream(x));
+      pre.defined() ? q(pre) : nullptr, M, E, I, O, (int)act, code(x), wp(ws),
+      stream(x));
   return pre.defined() ? pair(y, pre, false) : out(y);
 }
 
@@ -443,14 +455,14 @@ PyObject* grouped_linear_backward(const Args& a) {
   const int64_t xs = row_stride(x, "x");
   const c10::DeviceGuard guard(x.device());
   // the library writes dw with the input dimension contiguous where the weight's is
-  Tensor dx = make(x, {M, I}), dw = weight_grad(w, si != 1), db, ws;
+  Tensor dx = make(x, {M, I}), dw = weight_grad(w, si != 1), db;
   if (a.i64(7)) db = make(x, {E, O});
-  const int64_t bytes =
-      pulsar_grouped_linear_backward_workspace_bytes(M, E, I, O, (int)act, code(x));
-  if (bytes > 0) ws = make(x, {bytes}, at::kByte);
+  const Tensor ws = workspace(x, pulsar_grouped_linear_backward_workspace_bytes(
+      dy.data_ptr(), x.data_ptr(), xs, x.size(0), w.data_ptr(), w.stride(0), si, so, M, E, I, O,
+      (int)act, code(x)));
   run(pulsar_grouped_linear_backward, p(dy), p(x), xs, x.size(0), p<int32_t>(idx), p<int32_t>(off),
       p(w), w.stride(0), si, so, p(pre), q(dx), q(dw), db.defined() ? q(db) : nullptr, M, E, I, O,
-      (int)act, code(x), const_cast<void*>(p(ws)), stream(x));
+      (int)act, code(x), wp(ws), stream(x));
   return triple(dx, dw, db, true);
 }
 

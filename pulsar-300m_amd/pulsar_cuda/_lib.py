@@ -117,17 +117,22 @@ _PROTOS = {
                                          ctypes.c_int, _vp],
     "pulsar_moe_group_rows_workspace_bytes": [_c_i64] * 3,
     "pulsar_moe_group_rows": [_vp] * 4 + [_c_i64] * 3 + [_vp, _vp],
+    "pulsar_fused_linear_forward_workspace_bytes": [_vp, _c_i64, _vp] + [_c_i64] * 5 + [ctypes.c_int] * 2,
     "pulsar_fused_linear_forward": [_vp, _c_i64, _vp, _c_i64, _c_i64, _vp, ctypes.c_int, _vp,
                                     _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, ctypes.c_int,
-                                    ctypes.c_int, _vp],
-    "pulsar_fused_linear_backward_workspace_bytes": [_c_i64] * 3 + [ctypes.c_int] * 2,
+                                    ctypes.c_int, _vp, _vp],
+    "pulsar_fused_linear_backward_workspace_bytes": [_vp, _vp, _c_i64, _vp] + [_c_i64] * 5
+                                                    + [ctypes.c_int] * 2,
     "pulsar_fused_linear_backward": [_vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
                                      _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, _vp,
                                      _vp],
+    "pulsar_grouped_linear_forward_workspace_bytes": [_vp, _c_i64, _c_i64, _vp] + [_c_i64] * 7
+                                                     + [ctypes.c_int] * 2,
     "pulsar_grouped_linear_forward": [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64,
                                       _vp, ctypes.c_int, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
-                                      ctypes.c_int, ctypes.c_int, _vp],
-    "pulsar_grouped_linear_backward_workspace_bytes": [_c_i64] * 4 + [ctypes.c_int] * 2,
+                                      ctypes.c_int, ctypes.c_int, _vp, _vp],
+    "pulsar_grouped_linear_backward_workspace_bytes": [_vp, _vp, _c_i64, _c_i64, _vp] + [_c_i64] * 7
+                                                      + [ctypes.c_int] * 2,
     "pulsar_grouped_linear_backward": [_vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64,
                                        _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
                                        ctypes.c_int, ctypes.c_int, _vp, _vp],
@@ -153,7 +158,9 @@ _PROTOS = {
 # entries whose result is not an int status
 _RESTYPES = {name: _c_i64 for name in (
     "pulsar_sample_workspace_bytes", "pulsar_moe_router_workspace_bytes",
-    "pulsar_moe_group_rows_workspace_bytes", "pulsar_fused_linear_backward_workspace_bytes",
+    "pulsar_moe_group_rows_workspace_bytes", "pulsar_fused_linear_forward_workspace_bytes",
+    "pulsar_fused_linear_backward_workspace_bytes",
+    "pulsar_grouped_linear_forward_workspace_bytes",
     "pulsar_grouped_linear_backward_workspace_bytes")}
 
 EXPORTED = tuple(["pulsar_last_error", *_PROTOS])

@@ -142,27 +142,44 @@ def test_c_entries_refuse_before_any_launch():
     refused(lib.pulsar_moe_group_rows(p, p, p, p, 16384, 4, 16, None, None), b"workspace")
 
     def fwd(x=p, x_rs=8, w=p, w_out=8, w_in=1, y=p, rows=4, d_in=8, d_out=6, act=0, dt=bf, bias=None,
-            bdt=0):
+            bdt=0, ws=None):
         return lib.pulsar_fused_linear_forward(x, x_rs, w, w_out, w_in, bias, bdt, None, 0, y, None,
-                                               rows, d_in, d_out, act, dt, None)
+                                               rows, d_in, d_out, act, dt, ws, None)
 
     for kw, msg in ((dict(x=None), b"null"), (dict(w=None), b"null"), (dict(y=None), b"null"),
                     (dict(dt=5), b"dtype"), (dict(act=7), b"activation"), (dict(act=-1), b"activation"),
                     (dict(act=6, d_out=5), b"even"), (dict(w_in=2, w_out=16), b"strides"),
                     (dict(w_out=7), b"overlap"), (dict(w_out=0), b"overlap"), (dict(x_rs=7), b"overlap"),
                     (dict(rows=-1), b"shape"), (dict(d_in=0), b"shape"), (dict(d_out=0), b"shape"),
-                    (dict(rows=2 ** 31), b"shape"), (dict(bias=p, bdt=9), b"bias dtype")):
+                    (dict(rows=2 ** 31), b"shape"), (dict(bias=p, bdt=9), b"bias dtype"),
+                    (dict(x_rs=9), b"workspace"), (dict(d_in=7), b"workspace"),
+                    (dict(x_rs=9, ws=p.value + 8), b"workspace")):
         refused(fwd(**kw), msg)
     assert fwd(rows=0, x=None) == 0
-    n = lib.pulsar_fused_linear_backward_workspace_bytes(4, 8, 6, 2, bf)
-    assert n >= 4 * 6 * 2
+    odd = p.value + 2
+
+    def fwd_bytes(x=p, x_rs=8, w=p, w_out=8, w_in=1, rows=4, d_in=8, d_out=6, act=0):
+        return lib.pulsar_fused_linear_forward_workspace_bytes(x, x_rs, w, w_out, w_in, rows, d_in,
+                                                               d_out, act, bf)
+
+    # whole aligned rows need none; a copy is padded to chunks of 8 elements and 256 bytes
+    assert fwd_bytes() == 0 and fwd_bytes(rows=0, x=odd) == 0
+    assert fwd_bytes(x=odd) == 256 and fwd_bytes(x_rs=9) == 256 and fwd_bytes(w=odd) == 256
+    assert fwd_bytes(d_in=7, rows=100) == 100 * 16 + 192 + 256
+    assert fwd_bytes(w_out=1, w_in=8) == 256 and fwd_bytes(w_out=1, w_in=8, d_out=8) == 0
+    assert fwd_bytes(w_out=1, w_in=8, d_out=8, act=6) == 256
+    assert fwd_bytes(d_out=0) == -1 and fwd_bytes(act=9) == -1
+    n = lib.pulsar_fused_linear_backward_workspace_bytes(p, p, 8, p, 8, 1, 4, 8, 6, 2, bf)
+    assert n == 256
     refused(lib.pulsar_fused_linear_backward(p, p, 8, p, 8, 1, p, p, p, None, 4, 8, 6, 2, bf, None,
                                              None), b"workspace")
     refused(lib.pulsar_fused_linear_backward(p, p, 8, p, 8, 1, None, p, p, None, 4, 8, 6, 2, bf, p,
                                              None), b"null")
     refused(lib.pulsar_grouped_linear_forward(p, 8, 4, None, None, p, 48, 6, 1, None, 0, p, None, 4,
-                                              2, 8, 6, 0, bf, None), b"null")
+                                              2, 8, 6, 0, bf, None, None), b"null")
     refused(lib.pulsar_grouped_linear_forward(p, 8, 4, None, p, p, 48, 6, 1, None, 0, p, None, 4,
-                                              0, 8, 6, 0, bf, None), b"shape")
+                                              0, 8, 6, 0, bf, None, None), b"shape")
+    refused(lib.pulsar_grouped_linear_forward(p, 8, 4, None, p, p, 48, 6, 1, None, 0, p, None, 4,
+                                              2, 8, 6, 0, bf, None, None), b"workspace")
     refused(lib.pulsar_grouped_linear_backward(p, p, 8, 4, None, None, p, 48, 6, 1, None, p, p, None,
                                                4, 2, 8, 6, 0, bf, None, None), b"null")
