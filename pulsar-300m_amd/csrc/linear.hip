@@ -73,15 +73,11 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
   typedef typename Frag<T>::type F;
   const Reader<T, BM, true, PLAIN, 1> ra(row_w);
   const Reader<T, BN, BKC, MAP, BW> rb(col_w), ru(OBN + col_w);
-  auto rd = [&](const uint4* la, const uint4* lb, int s, F(&fa)[RT], F(&fb)[CT], int part) {
-    if (part == 0) {
-      rb.template read<NCT>(lb, s, fb);
-      if constexpr (PAIR) ru.template read<NCT>(lb, s, fb + NCT);
-    } else {
-      ra.template read<RT>(la, s, fa);
-    }
+  auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) {
+    rb.template read<NCT>(lb, s, fb);
+    if constexpr (PAIR) ru.template read<NCT>(lb, s, fb + NCT);
   };
-  pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, rd, [](int, F(&)[RT], F(&)[CT]) {});
+  pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, ra, read_b, [](int, const F&, F(&)[CT]) {});
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   rows_epilogue<T, MAP, BW, PAIR>(a, acc, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats, group, none,
@@ -91,14 +87,14 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
 // Weight gradient: C_group[m][n] = sum over the group's rows r of A[r][m] B[r][n], rows through
 // the optional indices. SIDE: the operand whose column sums (the bias gradient) are taken
 // along, by one more product with ones in the tiles at 0 of the other dimension (0 none, 1 A,
-// 2 B).
-template <typename T, int SIDE, typename SH>
+// 2 B). ROWS: the operand whose rows an index names, likewise.
+template <typename T, int SIDE, int ROWS, typename SH>
 __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(LinearArgs a) {
   constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
   constexpr Map MAP = out_map<T, false>();
   constexpr int BWR = RT >= 4 ? 4 : 2, BWC = CT >= 4 ? 4 : 2;
-  typedef Operand<T, BM, false, MAP, SH::kThreads> OA;
-  typedef Operand<T, BN, false, MAP, SH::kThreads> OB;
+  typedef Operand<T, BM, false, MAP, SH::kThreads, ROWS == 1> OA;
+  typedef Operand<T, BN, false, MAP, SH::kThreads, ROWS == 2> OB;
   __shared__ uint4 lds[2 * (OA::kChunks + OB::kChunks)];
   uint4 *sA = lds, *sB = lds + 2 * OA::kChunks;
   static_assert(sizeof(lds) >= SH::WR * SH::WC * Slab<CT>::kFloats * 4, "the epilogue's slabs fit");
@@ -149,15 +145,10 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
   typedef typename Frag<T>::type F;
   const Reader<T, BM, false, MAP, BWR> ra(row_w);
   const Reader<T, BN, false, MAP, BWC> rb(col_w);
-  auto rd = [&](const uint4* la, const uint4* lb, int s, F(&fa)[RT], F(&fb)[CT], int part) {
-    if (part == 0)
-      rb.template read<CT>(lb, s, fb);
-    else
-      ra.template read<RT>(la, s, fa);
-  };
-  auto extra = [&](int i, F(&fa)[RT], F(&fb)[CT]) {
+  auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) { rb.template read<CT>(lb, s, fb); };
+  auto extra = [&](int i, const F& fa, F(&fb)[CT]) {
     if constexpr (SIDE == 1) {
-      if (sums) sum[i] = mma(ones, fa[i], sum[i]);
+      if (sums) sum[i] = mma(ones, fa, sum[i]);
     }
     if constexpr (SIDE == 2) {
       if (sums && i == 0)
@@ -165,7 +156,7 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
         for (int j = 0; j < CT; ++j) sum[j] = mma(fb[j], ones, sum[j]);
     }
   };
-  pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, rd, extra);
+  pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, ra, read_b, extra);
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats,
@@ -363,12 +354,21 @@ int launch_wgrad(LinearArgs& a, int side, hipStream_t s) {
   if (tiles > (int64_t)1 << 30) return fail(PULSAR_ERR_INVALID, "linear: launch too large");
   const int64_t run = kXcds * std::max<int64_t>(1, per / kXcds);  // place_wgrad's
   const unsigned grid = (unsigned)((tiles + run - 1) / run * run);
+  auto go = [&](auto sd) {
+    constexpr int S = decltype(sd)::value;
+    if (a.a_rows)
+      linear_wgrad_kernel<T, S, 1, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    else if (a.b_rows)
+      linear_wgrad_kernel<T, S, 2, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    else
+      linear_wgrad_kernel<T, S, 0, SH><<<grid, SH::kThreads, 0, s>>>(a);
+  };
   if (side == 0)
-    linear_wgrad_kernel<T, 0, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    go(std::integral_constant<int, 0>{});
   else if (side == 1)
-    linear_wgrad_kernel<T, 1, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    go(std::integral_constant<int, 1>{});
   else
-    linear_wgrad_kernel<T, 2, SH><<<grid, SH::kThreads, 0, s>>>(a);
+    go(std::integral_constant<int, 2>{});
   PULSAR_LAUNCH_CHECK();
   if (a.splits > 1) {
     const int64_t n_c = (int64_t)a.groups * a.M * a.N;
@@ -487,6 +487,9 @@ struct Call {
   int check() const {
     const int rc = check_common(rows, groups, d_in, d_out, w, act, dtype, what);
     if (rc != PULSAR_OK) return rc;
+    // the kernels multiply row indexes and strides in 32 bits
+    if (x_rs > 0x7fffffff || w.in > 0x7fffffff || w.out > 0x7fffffff)
+      return fail(PULSAR_ERR_INVALID, std::string(what) + ": row strides must be below 2^31 elements");
     if (x_rows < 0 || (rows > 0 && x_rs < d_in && x_rows > 1))
       return fail(PULSAR_ERR_INVALID, std::string(what) + ": rows of x overlap");
     return PULSAR_OK;

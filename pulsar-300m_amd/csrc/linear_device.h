@@ -53,8 +53,9 @@ enum Map { PLAIN, WIDE, BLOCK };
 //     c ^ key(r), which spreads the 16 rows a fragment read takes over the banks.
 //   otherwise (rows of R contiguous elements per k): LDS [k][R]. bf16 tiles are read through
 //     the LDS transpose load, 4 k rows x 32 bytes per 16 lanes: 32-byte pairs of chunks sit
-//     at pair ^ (k & 3), which puts the 4 rows on different banks.
-template <typename T, int R, bool KC, Map MAP, int THREADS>
+//     at pair ^ (k & 3), which puts the 4 rows on different banks. ROWS: k row r is stored row
+//     k_rows[r].
+template <typename T, int R, bool KC, Map MAP, int THREADS, bool ROWS = false>
 struct Operand {
   static constexpr int EV = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
   static constexpr int kChunks = R * 8, NCH = kChunks / THREADS;
@@ -63,12 +64,12 @@ struct Operand {
 
   const T* base[KC ? NCH : 1];
   int64_t ld;             // !KC: elements from k to k + 1
-  const int32_t* k_rows;  // !KC: stored row of each k (nullptr: k itself)
+  const int32_t* k_rows;  // ROWS: stored row of each k
   int64_t k_nrows;
   uint32_t ok;            // KC: rows that exist
   int off;                // KC: first k of this thread's chunks; else: its first k row
   bool valid;             // !KC: this thread's chunk columns lie inside the matrix
-  int index;              // !KC with k_rows: the lane's row of the step to be loaded next
+  int index;              // ROWS: the lane's row of the step to be loaded next
 
   __device__ __forceinline__ static int key(int r) {
     if constexpr (MAP == WIDE) return (r & 3) | ((r >> 3 & 1) << 2);
@@ -104,8 +105,7 @@ struct Operand {
   }
   // Reads the row indices of step k0, a lane each, one step ahead of the loads that use them.
   __device__ __forceinline__ void prefetch(int k0, int K) {
-    if constexpr (!KC) {
-      if (!k_rows) return;
+    if constexpr (ROWS) {
       static_assert(BK <= 64, "a lane per k");
       const int k = k0 + ((int)threadIdx.x & 63);
       index = k < K ? k_rows[k] : -1;
@@ -122,12 +122,15 @@ struct Operand {
     } else {
       const int k = k0 + off + i * (THREADS * EV / R);
       in = valid && k < K;
-      int64_t r = k;
-      if (k_rows) {
-        r = __shfl(index, off + i * (THREADS * EV / R), 64);
-        in = in && r >= 0 && r < k_nrows;
+      if constexpr (ROWS) {
+        // a row index outside the matrix, negative ones too, is past its rows as an unsigned one;
+        // strides fit 32 bits
+        const uint32_t r = (uint32_t)__shfl(index, off + i * (THREADS * EV / R), 64);
+        in = in && r < (uint64_t)k_nrows;
+        p = base[0] + (uint64_t)r * (uint32_t)ld;
+      } else {
+        p = base[0] + (int64_t)k * ld;
       }
-      p = base[0] + r * ld;
     }
     const uint32_t w = __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63);
     load_lds16_at(in ? (const void*)p : (const void*)&kZeroChunk, lds + (w + i * THREADS) * 16);
@@ -154,6 +157,7 @@ struct Frag<float> { typedef lin_f32x4 type; };
 // The lane's part of the LDS addresses is computed once; tiles and halves differ by constants.
 template <typename T, int R, bool KC, Map MAP, int BW>
 struct Reader {
+  static constexpr int kTiles = MAP == BLOCK ? BW : 1;  // of one read_at
   static constexpr int NV = KC ? 2 : sizeof(T) == 2 ? 4 : 1;
   int off[NV];  // bytes
   __device__ __forceinline__ explicit Reader(int row0) {
@@ -176,33 +180,36 @@ struct Reader {
   }
   template <int NT>
   __device__ __forceinline__ void read(const uint4* lds, int s, typename Frag<T>::type* f) const {
+#pragma unroll
+    for (int t = 0; t < NT; t += MAP == BLOCK ? BW : 1) read_at(lds, s, t, f + t);
+  }
+  // Tile t (BLOCK: the BW tiles from it).
+  __device__ __forceinline__ void read_at(const uint4* lds, int s, int t,
+                                          typename Frag<T>::type* f) const {
     const char* l = reinterpret_cast<const char*>(lds);
+    if constexpr (KC) {
+      const int d = map_row<MAP, BW>(t, 0) * 128;
+      *f = *reinterpret_cast<const typename Frag<T>::type*>(l + off[s] + d);
+    } else if constexpr (sizeof(T) == 2) {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s4* lds_s4;
+      const char* p = l + off[t & 3] + 32 * s * (R * 2) + (t >> 2) * 128;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * (R * 2)));
+      *f = __builtin_bit_cast(lin_bf16x8,
+                                __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
 #pragma unroll
-    for (int t = 0; t < NT; t += MAP == BLOCK ? BW : 1) {
-      if constexpr (KC) {
-        const int d = map_row<MAP, BW>(t, 0) * 128;
-        f[t] = *reinterpret_cast<const typename Frag<T>::type*>(l + off[s] + d);
-      } else if constexpr (sizeof(T) == 2) {
-        typedef short s4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s4* lds_s4;
-        const char* p = l + off[t & 3] + 32 * s * (R * 2) + (t >> 2) * 128;
-        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * (R * 2)));
-        f[t] = __builtin_bit_cast(lin_bf16x8,
-                                  __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      } else {
+      for (int j = 0; j < 4; ++j) {
+        const char* p = l + off[0] + ((16 * s + j) * R + 16 * t) * 4;
+        if constexpr (BW == 4) {
+          const lin_f32x4 v = *reinterpret_cast<const lin_f32x4*>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const char* p = l + off[0] + ((16 * s + j) * R + 16 * t) * 4;
-          if constexpr (BW == 4) {
-            const lin_f32x4 v = *reinterpret_cast<const lin_f32x4*>(p);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) f[t + b][j] = v[b];
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(p);
-            f[t][j] = v.x;
-            f[t + 1][j] = v.y;
-          }
+          for (int b = 0; b < 4; ++b) f[b][j] = v[b];
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(p);
+          f[0][j] = v.x;
+          f[1][j] = v.y;
         }
       }
     }
@@ -218,29 +225,46 @@ __device__ __forceinline__ lin_f32x4 mma(lin_f32x4 a, lin_f32x4 b, lin_f32x4 c) 
   return c;
 }
 
-// The main loop with direct loads: acc += A tile . B tile^T over K, B as the matrix core's first
-// operand, so that a lane ends with 4 consecutive n of its own m.
+// The main loop: acc += A tile . B tile^T over K, B as the matrix core's first operand, so that a
+// lane ends with 4 consecutive n of its own m.
 //
-// A step is 128 bytes of k in two halves. While a half is multiplied, the other half's fragments
-// are read from LDS into a second set of registers. After a step's first half nobody needs its
-// buffer any more: one barrier there frees it for the loads of the step after next, which are
-// issued between the second half's products and have a step and a half to arrive, and makes
-// the next step's buffer, loaded by then, visible. rd(la, lb, s, fa, fb, part): part 0 or 1 of
-// the fragment reads of half s. extra(i, fa, fb): more products with row tile i.
-template <typename T, typename SH, typename OA, typename OB, typename RD, typename EX>
+// A step is 128 bytes of k in two halves. While a half is multiplied, the next one's fragments
+// are read from LDS: B's into a second set of registers, those of A's row tile i into its own
+// as soon as its products are issued (the last tile alternates with a spare, so that its read
+// need not wait for the half's end). After a step's first half nobody needs its buffer any
+// more: one barrier there frees it for the loads of the step after next, which are issued
+// between the second half's products and have a step and a half to arrive, and makes the next
+// step's buffer, loaded by then, visible. extra(i, fa, fb): more products with row tile i.
+template <typename T, typename SH, typename OA, typename OB, typename RA, typename RB, typename EX>
 __device__ __forceinline__ void pipe_loop(OA& oa, OB& ob, int K, uint4* sA, uint4* sB,
-                                          lin_f32x4 (&acc)[SH::RT][SH::CT], RD&& rd, EX&& extra) {
+                                          lin_f32x4 (&acc)[SH::RT][SH::CT], const RA& ra, RB&& rb,
+                                          EX&& extra) {
   constexpr int RT = SH::RT, CT = SH::CT, BK = OA::BK, LA = OA::NCH, LB = OB::NCH;
+  constexpr int AT = RA::kTiles;  // tiles one read of A yields
   typedef typename Frag<T>::type F;
   const int steps = (K + BK - 1) / BK;
   if (steps == 0) return;
   const uint32_t da = lds_address(sA), db = lds_address(sB);
-  F fa0[RT], fb0[CT], fa1[RT], fb1[CT];
-  auto multiply = [&](int i, F(&fa)[RT], F(&fb)[CT]) {
+  F fa[RT], spare[AT], fb0[CT], fb1[CT];
+  // one half: products of (fa, with the last tiles in `last`) and fb; reads half s of (la, lb) into
+  // (fa, with the last tiles in `next_last`) and nb
+  auto half = [&](F(&fb)[CT], F(&nb)[CT], F* last, F* next_last, const uint4* la, const uint4* lb,
+                  int s, auto&& load) {
 #pragma unroll
-    for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
-    extra(i, fa, fb);
-    __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < RT; ++i) {
+      if (i == 0) {
+        rb(lb, s, nb);
+        ra.read_at(la, s, RT - AT, next_last);
+      } else if (i % AT == 0) {
+        ra.read_at(la, s, i - AT, fa + i - AT);
+      }
+      load(i);
+      const F& f = i < RT - AT ? fa[i] : last[i - (RT - AT)];
+#pragma unroll
+      for (int j = 0; j < CT; ++j) acc[i][j] = mma(fb[j], f, acc[i][j]);
+      extra(i, f, fb);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   // steps past the end load zero chunks and are never multiplied: the loop has one form
 #pragma unroll
@@ -256,33 +280,23 @@ __device__ __forceinline__ void pipe_loop(OA& oa, OB& ob, int K, uint4* sA, uint
   ob.prefetch(2 * BK, K);
   wait_vmcnt<LA + LB>();
   lds_barrier();
-  rd(sA, sB, 0, fa0, fb0, 0);
-  rd(sA, sB, 0, fa0, fb0, 1);
+  rb(sB, 0, fb0);
+#pragma unroll
+  for (int i = 0; i < RT; i += AT) ra.read_at(sA, 0, i, fa + i);
 #pragma unroll 1
   for (int st = 0; st < steps; ++st) {
     const int x = st & 1, y = x ^ 1, k0 = (st + 2) * BK;
-    const uint4 *xa = sA + x * OA::kChunks, *xb = sB + x * OB::kChunks;
-    const uint4 *ya = sA + y * OA::kChunks, *yb = sB + y * OB::kChunks;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      if (i == 0) rd(xa, xb, 1, fa1, fb1, 0);
-      if (i == (RT > 2 ? 1 : 0)) rd(xa, xb, 1, fa1, fb1, 1);
-      multiply(i, fa0, fb0);
-    }
+    half(fb0, fb1, fa + RT - AT, spare, sA + x * OA::kChunks, sB + x * OB::kChunks, 1, [](int) {});
     wait_vmcnt<0>();
     lds_barrier();
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      if (i == 0) rd(ya, yb, 0, fa0, fb0, 0);
-      if (i == (RT > 2 ? 1 : 0)) rd(ya, yb, 0, fa0, fb0, 1);
+    half(fb1, fb0, spare, fa + RT - AT, sA + y * OA::kChunks, sB + y * OB::kChunks, 0, [&](int i) {
 #pragma unroll
       for (int c = i * LA / RT; c < (i + 1) * LA / RT; ++c)
         oa.fetch(c, k0, K, da + x * (OA::kChunks * 16));
 #pragma unroll
       for (int c = i * LB / RT; c < (i + 1) * LB / RT; ++c)
         ob.fetch(c, k0, K, db + x * (OB::kChunks * 16));
-      multiply(i, fa1, fb1);
-    }
+    });
     oa.prefetch(k0 + BK, K);
     ob.prefetch(k0 + BK, K);
   }
