@@ -59,21 +59,35 @@ __device__ __forceinline__ float fast_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504f));
 }
 
-// The activation of v, and its derivative.
-__device__ __forceinline__ float act_value(int act, float v) {
+// The activation of 8 values, chosen once for them.
+__device__ __forceinline__ void act_values(int act, float (&v)[8]) {
   switch (act) {
-    case PULSAR_ACT_RELU: return v < 0.f ? 0.f : v;  // NaN stays NaN
-    case PULSAR_ACT_SILU: return v * fast_sigmoid(v);
-    case PULSAR_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678f));
-    case PULSAR_ACT_GELU_TANH: {
+    case PULSAR_ACT_RELU:
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];  // NaN stays NaN
+      break;
+    case PULSAR_ACT_SILU:
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= fast_sigmoid(v[q]);
+      break;
+    case PULSAR_ACT_GELU:
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= 0.5f * (1.f + erff(v[q] * 0.70710678f));
+      break;
+    case PULSAR_ACT_GELU_TANH:
       // 0.5 (1 + tanh(u)) = sigmoid(2 u)
-      const float u = 0.79788456f * (v + 0.044715f * v * v * v);
-      return v * fast_sigmoid(2.f * u);
-    }
-    case PULSAR_ACT_SIGMOID: return fast_sigmoid(v);
-    default: return v;
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        v[q] *= fast_sigmoid(1.59576912f * (v[q] + 0.044715f * v[q] * v[q] * v[q]));
+      break;
+    case PULSAR_ACT_SIGMOID:
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = fast_sigmoid(v[q]);
+      break;
+    default: break;
   }
 }
+// The activation's derivative.
 // The slopes are taken at v held to a range past which they are 0 or 1 in fp32, so that no
 // infinite v meets a zero factor (NaN passes through).
 __device__ __forceinline__ float hold(float v, float b) { return v > b ? b : (v < -b ? -b : v); }

@@ -14,22 +14,22 @@ namespace {
 // tile's columns are BN / 2 gate columns and their up-projection twins.
 template <typename T, bool BKC, bool PAIR, typename SH>
 __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(LinearArgs a) {
-  constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
+  constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN, WAVES = SH::WR * SH::WC;
   constexpr Map MAP = out_map<T, BKC>();
   constexpr int NCT = PAIR ? CT / 2 : CT;  // tiles of output columns per wave
   constexpr int BW = NCT >= 4 ? 4 : 2;
-  static_assert(MAP == PLAIN || NCT % (MAP == WIDE ? 2 : BW) == 0, "whole runs per wave");
+  static_assert(CT == Slab::CT, "the epilogue's rows");
   typedef Operand<T, BM, true, PLAIN, SH::kThreads> OA;
   typedef Operand<T, BN, BKC, MAP, SH::kThreads> OB;
   __shared__ uint4 lds[2 * (OA::kChunks + OB::kChunks)];
   uint4 *sA = lds, *sB = lds + 2 * OA::kChunks;
-  static_assert(sizeof(lds) >= SH::WR * SH::WC * Slab<CT>::kFloats * 4, "the epilogue's slabs fit");
+  static_assert(sizeof(lds) >= WAVES * Slab::kFloats * 4, "the epilogue's rows fit");
 
   const int f = PAIR ? a.N / 2 : a.N;          // output columns
   constexpr int OBN = PAIR ? BN / 2 : BN;      // output columns of a tile
-  const int tiles_c = (f + OBN - 1) / OBN;
-  int tc, group, r0, r1;
-  if (!locate_tile<BM>(a, tiles_c, tc, group, r0, r1)) return;
+  int tr, tc, group, r0, r1;
+  RowTiles<BM> tiles(a);
+  if (!place_tile(tiles.total, (f + OBN - 1) / OBN, tr, tc) || !tiles.find(tr, group, r0, r1)) return;
   const int n0 = tc * OBN;
   const bool none = group >= a.groups;  // rows of no group: zeros
   const int K = none ? 0 : a.K;
@@ -60,16 +60,13 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
     });
   }
 
-  const int lane = (int)threadIdx.x & 63, wv = (int)threadIdx.x >> 6;
-  const int wr = wv / SH::WC, wc = wv % SH::WC;
-  const int i16 = lane & 15, kq = lane >> 4;
-  const int row_w = wr * RT * 16, col_w = wc * NCT * 16;
+  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int row_w = wv / SH::WC * RT * 16, col_w = wv % SH::WC * NCT * 16;
   lin_f32x4 acc[RT][CT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < CT; ++j) acc[i][j] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
-
   typedef typename Frag<T>::type F;
   const Reader<T, BM, true, PLAIN, 1> ra(row_w);
   const Reader<T, BN, BKC, MAP, BW> rb(col_w), ru(OBN + col_w);
@@ -80,8 +77,9 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
   pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, ra, read_b, [](int, const F&, F(&)[CT]) {});
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
-  rows_epilogue<T, MAP, BW, PAIR>(a, acc, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats, group, none,
-                                  r0 + row_w, r1, n0 + col_w, f);
+  const Slab slab{reinterpret_cast<float*>(lds) + wv * Slab::kFloats};
+  const EpilogueBias<T, MAP, PAIR> bias(a, group, none, n0 + col_w, f);
+  rows_epilogue<T, MAP, BW, PAIR>(a, acc, slab, bias, none, r0 + row_w, r1, n0 + col_w, f);
 }
 
 // Weight gradient: C_group[m][n] = sum over the group's rows r of A[r][m] B[r][n], rows through
@@ -97,7 +95,7 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
   typedef Operand<T, BN, false, MAP, SH::kThreads, ROWS == 2> OB;
   __shared__ uint4 lds[2 * (OA::kChunks + OB::kChunks)];
   uint4 *sA = lds, *sB = lds + 2 * OA::kChunks;
-  static_assert(sizeof(lds) >= SH::WR * SH::WC * Slab<CT>::kFloats * 4, "the epilogue's slabs fit");
+  static_assert(sizeof(lds) >= SH::WR * SH::WC * Slab::kFloats * 4, "the epilogue's rows fit");
 
   int group, split, mt, tc;
   if (!place_wgrad(a, group, split, mt, tc)) return;
@@ -159,8 +157,8 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
   pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, ra, read_b, extra);
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
-  wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum, reinterpret_cast<float*>(lds) + wv * Slab<CT>::kFloats,
-                                         sums, group, split, m0 + row_w, n0 + col_w);
+  const Slab slab{reinterpret_cast<float*>(lds) + wv * Slab::kFloats};
+  wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum, slab, sums, group, split, m0 + row_w, n0 + col_w);
 }
 
 // Sums of a weight gradient's splits, in order; `count` elements of one split's partials, the

@@ -315,52 +315,51 @@ __device__ __forceinline__ void group_span(const LinearArgs& a, int g, int& r0, 
   r1 = g < a.groups ? min(max(a.offsets[g + 1], 0), a.rows) : a.rows;
 }
 
-// The number of row tiles of the launch, counted group by group (64 at a time, one per lane), at
-// most the launch's bound.
+// Finds the row tiles of a launch, counted group by group, 64 groups at a time, one per lane. The
+// last of them are the rows of no group. With fewer than 64 groups (the usual case) the offsets
+// are looked at once.
 template <int BM>
-__device__ __forceinline__ int count_tiles(const LinearArgs& a) {
-  const int lane = (int)threadIdx.x & 63;
-  int64_t all = 0;
-  for (int g0 = 0; g0 <= a.groups; g0 += 64) {
-    int s0 = 0, s1 = 0;
-    if (g0 + lane <= a.groups) group_span(a, g0 + lane, s0, s1);
-    int nt = s1 > s0 ? (s1 - s0 + BM - 1) / BM : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) nt += __shfl_xor(nt, d, 64);
-    all += nt;
+struct RowTiles {
+  const LinearArgs& a;
+  int total;             // at most the launch's bound
+  int s0, s1, nt, incl;  // this lane's group of the 64 looked at: rows, tiles, tiles up to it
+  __device__ __forceinline__ explicit RowTiles(const LinearArgs& args) : a(args) {
+    int64_t all = 0;
+    for (int g0 = 0; g0 <= a.groups; g0 += 64) all += look(g0);
+    total = (int)min(all, (int64_t)a.max_tiles);
   }
-  return (int)min(all, (int64_t)a.max_tiles);
-}
-
-// Row tile t: its group, first row and the group's end. false: there is none.
-template <int BM>
-__device__ __forceinline__ bool find_tile(const LinearArgs& a, int t, int& group, int& r0, int& r1) {
-  const int lane = (int)threadIdx.x & 63;
-  int64_t before = 0;
-  for (int g0 = 0; g0 <= a.groups; g0 += 64) {
-    int s0 = 0, s1 = 0;
+  __device__ __forceinline__ int look(int g0) {
+    const int lane = (int)threadIdx.x & 63;
+    s0 = s1 = 0;
     if (g0 + lane <= a.groups) group_span(a, g0 + lane, s0, s1);
-    const int nt = s1 > s0 ? (s1 - s0 + BM - 1) / BM : 0;
-    int incl = nt;
+    nt = s1 > s0 ? (s1 - s0 + BM - 1) / BM : 0;
+    incl = nt;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int v = __shfl_up(incl, d, 64);
       if (lane >= d) incl += v;
     }
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (t < before + total) {
-      // the first lane whose inclusive count passes t
-      const int src = (int)__builtin_popcountll(__ballot(before + incl <= t));
-      group = g0 + src;
-      r1 = __builtin_amdgcn_readlane(s1, src);
-      r0 = __builtin_amdgcn_readlane(s0, src) +
-           (int)(t - before - __builtin_amdgcn_readlane(incl - nt, src)) * BM;
-      return true;
-    }
-    before += total;
+    return __builtin_amdgcn_readlane(incl, 63);
   }
-  return false;
-}
+  // Row tile t: its group, first row and the group's end. false: there is none.
+  __device__ __forceinline__ bool find(int t, int& group, int& r0, int& r1) {
+    int64_t before = 0;
+    for (int g0 = 0; g0 <= a.groups; g0 += 64) {
+      const int all = a.groups < 64 ? __builtin_amdgcn_readlane(incl, 63) : look(g0);
+      if (t < before + all) {
+        // the first lane whose inclusive count passes t
+        const int src = (int)__builtin_popcountll(__ballot(before + incl <= t));
+        group = g0 + src;
+        r1 = __builtin_amdgcn_readlane(s1, src);
+        r0 = __builtin_amdgcn_readlane(s0, src) +
+             (int)(t - before - __builtin_amdgcn_readlane(incl - nt, src)) * BM;
+        return true;
+      }
+      before += all;
+    }
+    return false;
+  }
+};
 
 // Tiles in the order that shares operands through one L2: the launch's tiles are cut into 8
 // contiguous ranges, one per XCD (workgroup L runs on XCD L % 8), and run in bands of kBand
@@ -373,41 +372,13 @@ __device__ __forceinline__ void band_tile(int item, int band_rows, int tiles_r, 
   tr = band * band_rows + in % rows;
   tc = in / rows;
 }
+// This workgroup's tile; false: it has none.
 __device__ __forceinline__ bool place_tile(int tiles_r, int tiles_c, int& tr, int& tc) {
-  const int total = tiles_r * tiles_c;
-  const int L = (int)blockIdx.x, xcd = L % kXcds, slot = L / kXcds;
-  const int per = (total + kXcds - 1) / kXcds;
-  const int item = xcd * per + slot;
+  const int total = tiles_r * tiles_c, xcd = (int)blockIdx.x % kXcds, slot = (int)blockIdx.x / kXcds;
+  const int per = (total + kXcds - 1) / kXcds, item = xcd * per + slot;
   if (slot >= per || item >= total) return false;
   band_tile(item, kBand, tiles_r, tiles_c, tr, tc);
   return true;
-}
-
-// The tile of this workgroup: column block tc, rows r0 .. of group `group`, whose end is r1.
-template <int BM>
-__device__ __forceinline__ bool locate_tile(const LinearArgs& a, int tiles_c, int& tc, int& group,
-                                            int& r0, int& r1) {
-  int tr;
-  if (a.groups < 64) {  // one look at the offsets (their loads are the start of every chain here)
-    const int lane = (int)threadIdx.x & 63;
-    int s0 = 0, s1 = 0;
-    if (lane <= a.groups) group_span(a, lane, s0, s1);
-    const int nt = s1 > s0 ? (s1 - s0 + BM - 1) / BM : 0;
-    int incl = nt;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += v;
-    }
-    const int tiles_r = min(__builtin_amdgcn_readlane(incl, 63), a.max_tiles);
-    if (!place_tile(tiles_r, tiles_c, tr, tc)) return false;
-    group = (int)__builtin_popcountll(__ballot(incl <= tr));
-    r1 = __builtin_amdgcn_readlane(s1, group);
-    r0 = __builtin_amdgcn_readlane(s0, group) +
-         (tr - __builtin_amdgcn_readlane(incl - nt, group)) * BM;
-    return true;
-  }
-  return place_tile(count_tiles<BM>(a), tiles_c, tr, tc) && find_tile<BM>(a, tr, group, r0, r1);
 }
 
 // Weight-gradient tiles: group by group, the largest groups first (up to 64 groups), so that the
@@ -481,38 +452,80 @@ constexpr Map out_map() {
   return KC ? (sizeof(T) == 2 ? WIDE : PLAIN) : (sizeof(T) == 2 ? PLAIN : BLOCK);
 }
 
-// Accumulators leave through LDS, two row tiles (32 rows) at a time in memory of the wave's own:
-// matrix-core order in, whole rows of C out, 8 columns a lane. Columns are read back in order,
-// so stores are 16 bytes and cover cache lines, and the epilogue is a short loop (unrolled
-// over the registers it was 15,000 instructions, which took longer to fetch than the tile's
-// products to run). Rows are 4 floats apart from a multiple of the banks.
-template <int CT>
-struct Slab {
-  static constexpr int kCols = 16 * CT, kStride = kCols + 4, kFloats = 32 * kStride;
-};
-
-// Writes one row tile of accumulators: LDS row i16, columns in order.
-template <Map MAP, int BW, int NCT, int CT>
-__device__ __forceinline__ void slab_write_tile(float* slab, const lin_f32x4 (&acc)[CT]) {
-  const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
+// bf16 results leave the matrix core's layout in registers: of a pair of column tiles, lane group
+// kq (16 lanes, a row each) ends with 8 consecutive columns, 16 bytes to store, 64 bytes a row
+// beside the other groups. WIDE tiles come that way; of PLAIN ones group kq holds columns 4 kq
+// .. of both tiles, and exchanging the odd groups of the first with the even ones of the second
+// leaves tile kq % 2, columns 8 (kq / 2) ...
+template <Map MAP>
+__device__ __forceinline__ int run_col(int kq) { return MAP == WIDE ? 8 * kq : 16 * (kq & 1) + 8 * (kq >> 1); }
+template <Map MAP>
+__device__ __forceinline__ void take_run(const lin_f32x4& x, const lin_f32x4& y, float (&v)[8]) {
+  static_assert(MAP != BLOCK, "bf16 tiles");
 #pragma unroll
-  for (int j = 0; j < CT; ++j) {
-    // tiles beyond NCT are the second set of a pair, 16 NCT columns on
-    const int u = j % NCT;
-    float* p = slab + i16 * Slab<CT>::kStride + j / NCT * 16 * NCT;
-    if constexpr (MAP == BLOCK) {
-      // element e of tile u: column 16 BW (u / BW) + BW (4 kq + e) + u % BW
-      if (u % BW) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int b = 0; b < BW; ++b) p[16 * u + BW * (4 * kq + e) + b] = acc[j + b][e];
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (MAP == WIDE) {
+      v[e] = x[e];
+      v[4 + e] = y[e];
     } else {
-      // 4 consecutive columns
-      *reinterpret_cast<lin_f32x4*>(p + map_row<MAP, BW>(u, 0) + (MAP == WIDE ? 8 : 4) * kq) = acc[j];
+      const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[e]), __float_as_uint(y[e]),
+                                                      false, false);
+      v[e] = __uint_as_float(s[0]);
+      v[4 + e] = __uint_as_float(s[1]);
     }
   }
 }
+
+// fp32 results, and those of the erf activation (280 instructions a run: unrolled over the
+// accumulators they take longer to fetch than the products to run), leave through LDS, a row tile
+// at a time in memory of the wave's own: matrix-core order in, whole rows of C out, 8 columns a
+// lane, in a short loop. A row's 16-byte chunks sit at chunk ^ row, so that the 16 rows of a
+// column are on different banks. 256 x 256 tiles: 10 us this way, 5 from registers.
+struct Slab {
+  static constexpr int CT = 4, kFloats = 16 * 16 * CT;
+  float* l;
+  __device__ __forceinline__ lin_f32x4& chunk(int row, int c) const {
+    return reinterpret_cast<lin_f32x4*>(l)[row * 4 * CT + (c ^ row)];
+  }
+  // Writes a row tile's accumulators, columns in order; tiles beyond NCT are the second set of a
+  // pair, 16 NCT columns on.
+  template <Map MAP, int BW, int NCT>
+  __device__ __forceinline__ void write(const lin_f32x4 (&acc)[CT]) const {
+    const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const int set = 4 * NCT * (j / NCT), u = j % NCT;
+      if constexpr (MAP == BLOCK) {
+        // element e of tiles u .. u + BW - 1: columns 16 u + BW (4 kq + e) ..
+        if (u % BW) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (BW == 4) {
+            chunk(i16, set + 4 * u + 4 * kq + e) = lin_f32x4{acc[j][e], acc[j + 1][e], acc[j + 2][e], acc[j + 3][e]};
+          } else {
+            float* p = reinterpret_cast<float*>(&chunk(i16, set + 4 * u + 2 * kq + e / 2)) + 2 * (e & 1);
+            p[0] = acc[j][e];
+            p[1] = acc[j + 1][e];
+          }
+        }
+      } else if constexpr (MAP == WIDE) {
+        chunk(i16, set + 8 * (u / 2) + 2 * kq + (u & 1)) = acc[j];
+      } else {
+        chunk(i16, set + 4 * u + kq) = acc[j];
+      }
+    }
+  }
+  __device__ __forceinline__ void read8(int row, int c, float (&v)[8]) const {
+    const lin_f32x4 x = chunk(row, c), y = chunk(row, c + 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[q] = x[q];
+      v[4 + q] = y[q];
+    }
+  }
+};
+// Between a wave's own writes and reads of LDS.
+__device__ __forceinline__ void lds_settle() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // The bias of 8 columns, of both halves for a pair.
 template <bool PAIR>
@@ -535,70 +548,183 @@ __device__ __forceinline__ void load_bias(const LinearArgs& a, int group, bool n
 }
 
 // 8 columns of row r from their sums v (and u, a pair's second half): bias, activation and
-// residual in fp32, one rounding per output.
+// residual in fp32. Leaves the pre-activation values in `pre` (and u), the results in v.
 template <typename T, bool PAIR>
-__device__ __forceinline__ void finish_run(const LinearArgs& a, int act, int64_t r, int col, int f,
-                                           float (&v)[8], float (&u)[8], const float (&bias)[2][8]) {
-  const int n = f - col;
+__device__ __forceinline__ void finish_values(const LinearArgs& a, int act, int64_t r, int col, int f,
+                                              float (&v)[8], float (&u)[8], float (&pre)[8],
+                                              const float (&bias)[2][8]) {
+  if (a.bias) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    v[q] += bias[0][q];
-    if constexpr (PAIR) u[q] += bias[1][q];
+    for (int q = 0; q < 8; ++q) {
+      v[q] += bias[0][q];
+      if constexpr (PAIR) u[q] += bias[1][q];
+    }
   }
-  if (a.pre) {
-    T* pre = reinterpret_cast<T*>(a.pre) + r * a.ldpre + col;
-    store_run<8>(pre, v, n);
-    if constexpr (PAIR) store_run<8>(pre + f, u, n);
-  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) pre[q] = v[q];
   if constexpr (PAIR) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = v[q] * fast_sigmoid(v[q]) * u[q];
-  } else if (act != PULSAR_ACT_NONE) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = act_value(act, v[q]);
+  } else {
+    act_values(act, v);
   }
   if (a.residual) {
     float x[8];
-    load_run<8>(reinterpret_cast<const T*>(a.residual) + r * a.ldr + col, x, n);
+    load_run<8>(reinterpret_cast<const T*>(a.residual) + r * a.ldr + col, x, f - col);
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] += x[q];
+  }
+}
+// The same, stored with one rounding.
+template <typename T, bool PAIR>
+__device__ __forceinline__ void finish_run(const LinearArgs& a, int act, int64_t r, int col, int f,
+                                           float (&v)[8], float (&u)[8], const float (&bias)[2][8]) {
+  float pre[8];
+  finish_values<T, PAIR>(a, act, r, col, f, v, u, pre, bias);
+  const int n = f - col;
+  if (a.pre) {
+    T* o = reinterpret_cast<T*>(a.pre) + r * a.ldpre + col;
+    store_run<8>(o, pre, n);
+    if constexpr (PAIR) store_run<8>(o + f, u, n);
   }
   store_run<8>(reinterpret_cast<T*>(a.C) + r * a.ldc + col, v, n);
 }
 
-// Epilogue of a product's tile. The wave's accumulators start at row r0 and output column c0; of `f` output columns and rows
-// below r1 only those inside are stored. PAIR: the second half of the CT tiles are the
-// up-projection twins of the first.
-template <typename T, Map MAP, int BW, bool PAIR, int RT, int CT>
-__device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&acc)[RT][CT],
-                                              float* slab, int group, bool none, int r0, int r1,
-                                              int c0, int f) {
-  constexpr int NCT = PAIR ? CT / 2 : CT, LPR = NCT * 2, RPI = 64 / LPR;  // lanes a row, rows a pass
-  static_assert(64 % LPR == 0, "whole rows per pass");
-  const int lane = (int)threadIdx.x & 63, lc = (lane % LPR) * 8, lr = lane / LPR;
-  const int col = c0 + lc, n = f - col;
-  float bias[2][8];
-  load_bias<PAIR>(a, group, none, col, f, bias);
-  const int act = none ? PULSAR_ACT_NONE : a.act;
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < RT; i += 2) {
-    slab_write_tile<MAP, BW, NCT>(slab, acc[i]);
-    slab_write_tile<MAP, BW, NCT>(slab + 16 * Slab<CT>::kStride, acc[i + 1]);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-    for (int p = lr; p < 32; p += RPI) {
-      const int64_t r = r0 + 16 * i + p;
-      if (r >= r1 || n <= 0) continue;
-      float v[8], u[8];
-      const float* l = slab + p * Slab<CT>::kStride + lc;
+  for (int q = 0; q < 4; ++q) w[q] = (uint32_t)f2bf(v[2 * q]).u | ((uint32_t)f2bf(v[2 * q + 1]).u << 16);
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+
+// Stores two runs of a lane, as bf16, of columns c0 .. and 32 further on, in the wave's layout (row
+// i16, column run by lane group). Rows 0 - 7 give their second run for rows 8 - 15's first, so
+// that a store covers 8 rows by 128 bytes, whole cache lines, and not 16 by 64. With two waves
+// on a SIMD an instruction for each of a lane's 128 results is half a us of a tile: addresses
+// are one 64-bit addition a store, bounds are only looked at in tiles that have any.
+template <Map MAP>
+struct PairStore {
+  bf16* p;
+  int64_t ld;
+  int left, n;  // rows and columns inside from this lane's first
+  bool whole;   // of the wave's tile
+  __device__ __forceinline__ PairStore(bf16* m, int64_t ld_, int rows, int r0, int r1, int c0, int f) : ld(ld_) {
+    const int lane = (int)threadIdx.x & 63, i16 = lane & 15;
+    const int r = r0 + (i16 & 7), c = c0 + run_col<MAP>(lane >> 4) + (i16 >= 8 ? 32 : 0);
+    p = m + r * ld + c;
+    left = r1 - r;
+    n = f - c;
+    whole = r1 - r0 >= rows && f - c0 >= 64;
+  }
+  __device__ __forceinline__ void operator()(int i, const uint4& x, const uint4& y) const {
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    uint32_t w[2][4];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        v[q] = l[q];
-        u[q] = PAIR ? l[16 * NCT + q] : 0.f;
-      }
-      finish_run<T, PAIR>(a, act, r, col, f, v, u, bias);
+    for (int q = 0; q < 4; ++q) {
+      // lanes 8 - 15 of each 16: the other half's (row rotation by 8, written to banks 2 and 3)
+      w[0][q] = (uint32_t)__builtin_amdgcn_update_dpp((int)xs[q], (int)ys[q], 0x128, 0xf, 0xc, false);
+      w[1][q] = (uint32_t)__builtin_amdgcn_update_dpp((int)ys[q], (int)xs[q], 0x128, 0xf, 0x3, false);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next rows overwrite
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16* o = p + (16 * i + 8 * h) * ld;
+      if (whole || (16 * i + 8 * h < left && n >= 8)) {
+        __builtin_memcpy(o, w[h], 16);
+      } else if (16 * i + 8 * h < left) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < n) o[q].u = (uint16_t)(w[h][q >> 1] >> (16 * (q & 1)));
+      }
+    }
+  }
+};
+
+// The bias of the wave's columns as the epilogue will want them: of bf16 results runs of 8, from
+// column c0; of fp32 ones the lane's 8 of a slab row.
+template <typename T, Map MAP, bool PAIR>
+struct EpilogueBias {
+  static constexpr int NCT = PAIR ? Slab::CT / 2 : Slab::CT;
+  static constexpr int N = sizeof(T) == 2 ? NCT / 2 : 1;
+  float b[N][2][8], slab[2][8];
+  __device__ __forceinline__ EpilogueBias(const LinearArgs& a, int group, bool none, int c0, int f) {
+    const int lane = (int)threadIdx.x & 63;
+    const bool via_slab = sizeof(T) == 4 || a.act == PULSAR_ACT_GELU;
+    const int lc = c0 + lane % (NCT * 2) * 8;
+    load_bias<PAIR>(a, group, none || !via_slab, lc, f, slab);
+#pragma unroll
+    for (int p = 0; p < N; ++p) load_bias<PAIR>(a, group, none || via_slab, c0 + 32 * p + run_col<MAP>(lane >> 4), f, b[p]);
+  }
+};
+
+// Epilogue of a product's tile. The wave's accumulators start at row r0 and output column c0; of
+// `f` output columns and rows below r1 only those inside are stored. PAIR: the second half of the
+// CT tiles are the up-projection twins of the first.
+template <typename T, Map MAP, int BW, bool PAIR, int RT>
+__device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&acc)[RT][Slab::CT],
+                                              Slab slab, const EpilogueBias<T, MAP, PAIR>& bias,
+                                              bool none, int r0, int r1, int c0, int f) {
+  constexpr int NCT = PAIR ? Slab::CT / 2 : Slab::CT;
+  const int lane = (int)threadIdx.x & 63, act = none ? PULSAR_ACT_NONE : a.act;
+  if constexpr (sizeof(T) == 2 && !PAIR) {
+    const PairStore<MAP> out(reinterpret_cast<bf16*>(a.C), a.ldc, 16 * RT, r0, r1, c0, f);
+    if (act == PULSAR_ACT_NONE && !a.bias && !a.residual && !a.pre) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float v[2][8];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) take_run<MAP>(acc[i][2 * p], acc[i][2 * p + 1], v[p]);
+        out(i, pack8(v[0]), pack8(v[1]));
+      }
+      return;
+    }
+    if (act != PULSAR_ACT_GELU) {
+      const PairStore<MAP> kept(reinterpret_cast<bf16*>(a.pre), a.ldpre, 16 * RT, r0, r1, c0, f);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        // the residual's rows past the end: the last one's
+        const int64_t r = min(r0 + 16 * i + (lane & 15), r1 - 1);
+        uint4 o[2], k[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          float v[8], u[8], pre[8];
+          take_run<MAP>(acc[i][2 * p], acc[i][2 * p + 1], v);
+          finish_values<T, PAIR>(a, act, r, c0 + 32 * p + run_col<MAP>(lane >> 4), f, v, u, pre, bias.b[p]);
+          o[p] = pack8(v);
+          k[p] = pack8(pre);
+        }
+        if (a.pre) kept(i, k[0], k[1]);
+        out(i, o[0], o[1]);
+      }
+      return;
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const int col = c0 + run_col<MAP>(lane >> 4);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      float v[8], u[8];
+      take_run<MAP>(acc[i][0], acc[i][1], v);
+      take_run<MAP>(acc[i][2], acc[i][3], u);
+      const int64_t r = r0 + 16 * i + (lane & 15);
+      if (r < r1 && col < f) finish_run<T, PAIR>(a, act, r, col, f, v, u, bias.b[0]);
+    }
+    return;
+  }
+  constexpr int LPR = NCT * 2, RPI = 64 / LPR;  // lanes a row, rows a pass
+  const int lc = lane % LPR, lr = lane / LPR, col = c0 + 8 * lc;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    slab.write<MAP, BW, NCT>(acc[i]);
+    lds_settle();
+#pragma unroll 1
+    for (int p = lr; p < 16; p += RPI) {
+      const int64_t r = r0 + 16 * i + p;
+      if (r >= r1 || col >= f) continue;
+      float v[8], u[8] = {};
+      slab.read8(p, 2 * lc, v);
+      if constexpr (PAIR) slab.read8(p, 4 * NCT + 2 * lc, u);
+      finish_run<T, PAIR>(a, act, r, col, f, v, u, bias.slab);
+    }
+    lds_settle();  // read before the next rows overwrite
   }
 }
 
@@ -606,30 +732,44 @@ __device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&a
 // the column sums of SIDE's operand.
 template <typename T, Map MAP, int BWR, int BWC, int SIDE, int RT, int CT, int NS>
 __device__ __forceinline__ void wgrad_epilogue(const LinearArgs& a, lin_f32x4 (&acc)[RT][CT],
-                                               lin_f32x4 (&sum)[NS], float* slab, bool sums,
+                                               lin_f32x4 (&sum)[NS], Slab slab, bool sums,
                                                int group, int split, int m0, int n0) {
   const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
-  constexpr int LPR = CT * 2, RPI = 64 / LPR;
-  const int lc = (lane % LPR) * 8, lr = lane / LPR, col = n0 + lc, n = a.N - col;
   const int64_t pg = (int64_t)split * a.groups + group;  // a split's partial results
+  auto store = [&](int64_t m, int col, const float (&v)[8]) {
+    if (m >= a.M || col >= a.N) return;
+    if (a.splits > 1)
+      store_run<8>(a.part + (pg * a.M + m) * a.N + col, v, a.N - col);
+    else
+      store_run<8>(reinterpret_cast<T*>(a.C) + group * a.c_group + m * a.ldc + col, v, a.N - col);
+  };
+  if constexpr (sizeof(T) == 2) {
+    const PairStore<MAP> out(reinterpret_cast<bf16*>(a.C) + group * a.c_group, a.ldc, 16 * RT, m0, a.M, n0, a.N);
 #pragma unroll
-  for (int i = 0; i < RT; i += 2) {
-    slab_write_tile<MAP, BWC, CT>(slab, acc[i]);
-    slab_write_tile<MAP, BWC, CT>(slab + 16 * Slab<CT>::kStride, acc[i + 1]);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-    for (int p = lr; p < 32; p += RPI) {
-      const int64_t m = m0 + (p < 16 ? map_row<MAP, BWR>(i, p) : map_row<MAP, BWR>(i + 1, p - 16));
-      if (m >= a.M || n <= 0) continue;
-      float v[8];
+    for (int i = 0; i < RT; ++i) {
+      float v[2][8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = slab[p * Slab<CT>::kStride + lc + q];
-      if (a.splits > 1)
-        store_run<8>(a.part + (pg * a.M + m) * a.N + col, v, n);
-      else
-        store_run<8>(reinterpret_cast<T*>(a.C) + group * a.c_group + m * a.ldc + col, v, n);
+      for (int p = 0; p < 2; ++p) take_run<MAP>(acc[i][2 * p], acc[i][2 * p + 1], v[p]);
+      if (a.splits > 1) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) store(m0 + 16 * i + i16, n0 + 32 * p + run_col<MAP>(kq), v[p]);
+      } else {
+        out(i, pack8(v[0]), pack8(v[1]));
+      }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      slab.write<MAP, BWC, CT>(acc[i]);
+      lds_settle();
+#pragma unroll 1
+      for (int p = lane / 8; p < 16; p += 8) {
+        float v[8];
+        slab.read8(p, lane % 8 * 2, v);
+        store(m0 + map_row<MAP, BWR>(i, p), n0 + lane % 8 * 8, v);
+      }
+      lds_settle();
+    }
   }
   // SIDE 1: lane i16 holds row map_row(i, i16) of A in every element; SIDE 2: element e of lane
   // group kq holds row 4 kq + e of B's tile

@@ -14,6 +14,33 @@ __device__ __forceinline__ uint4 load_chunk(const void* p, bool in) {
   return r;
 }
 
+// Floats from one row of a workgroup's sums in LDS to the next: 4 apart from a multiple of the banks.
+template <int CT>
+constexpr int kSumStride = 16 * CT + 4;
+
+// Writes one row tile of accumulators: LDS row i16, columns in order.
+template <Map MAP, int BW, int NCT, int CT>
+__device__ __forceinline__ void slab_write_tile(float* slab, const lin_f32x4 (&acc)[CT]) {
+  const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < CT; ++j) {
+    // tiles beyond NCT are the second set of a pair, 16 NCT columns on
+    const int u = j % NCT;
+    float* p = slab + i16 * kSumStride<CT> + j / NCT * 16 * NCT;
+    if constexpr (MAP == BLOCK) {
+      // element e of tile u: column 16 BW (u / BW) + BW (4 kq + e) + u % BW
+      if (u % BW) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int b = 0; b < BW; ++b) p[16 * u + BW * (4 * kq + e) + b] = acc[j + b][e];
+    } else {
+      // 4 consecutive columns
+      *reinterpret_cast<lin_f32x4*>(p + map_row<MAP, BW>(u, 0) + (MAP == WIDE ? 8 : 4) * kq) = acc[j];
+    }
+  }
+}
+
 // A workgroup owns 16 RT rows of a group and 16 NCT output columns; its W waves take a run of k
 // each, with D steps of operands in flight in registers, and add their sums through LDS at the
 // end. Weights that are contiguous along k go from memory straight into matrix-core order; bf16
@@ -27,14 +54,15 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
   constexpr bool TR = !BKC && sizeof(T) == 2;
   constexpr Map MAP = !BKC && sizeof(T) == 4 ? BLOCK : PLAIN;
   constexpr int BW = NCT;
-  typedef Slab<CT> SL;
+  constexpr int SS = kSumStride<CT>;
   constexpr int kStage = TR ? CT * 64 : 1;  // chunks of a step's weights, per wave
-  constexpr int kBytes = 16 * W * kStage, kSums = W * BM * SL::kStride * 4;
+  constexpr int kBytes = 16 * W * kStage, kSums = W * BM * SS * 4;
   __shared__ __attribute__((aligned(16))) char lds[kBytes > kSums ? kBytes : kSums];
 
   const int f = PAIR ? a.N / 2 : a.N, tiles_c = (f + OBN - 1) / OBN;
-  int tc, group, r0, r1;
-  if (!locate_tile<BM>(a, tiles_c, tc, group, r0, r1)) return;
+  int tr, tc, group, r0, r1;
+  RowTiles<BM> tiles(a);
+  if (!place_tile(tiles.total, tiles_c, tr, tc) || !tiles.find(tr, group, r0, r1)) return;
   const bool none = group >= a.groups;
   const int n0 = tc * OBN;
   const int lane = (int)threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -169,12 +197,12 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
   // sums of the waves, in order
   __syncthreads();
   float* sums = reinterpret_cast<float*>(lds);
-  float* own = sums + wv * BM * SL::kStride;
+  float* own = sums + wv * BM * SS;
   if constexpr (RT == 1) {
     slab_write_tile<MAP, BW, NCT>(own, acc[0]);
   } else {
 #pragma unroll
-    for (int i = 0; i < RT; ++i) slab_write_tile<MAP, BW, NCT>(own + 16 * i * SL::kStride, acc[i]);
+    for (int i = 0; i < RT; ++i) slab_write_tile<MAP, BW, NCT>(own + 16 * i * SS, acc[i]);
   }
   __syncthreads();
   const int act = none ? PULSAR_ACT_NONE : a.act;
@@ -188,7 +216,7 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = u[q] = 0.f;
     for (int w = 0; w < W; ++w) {
-      const float* l = sums + (w * BM + p) * SL::kStride + lc;
+      const float* l = sums + (w * BM + p) * SS + lc;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         v[q] += l[q];
