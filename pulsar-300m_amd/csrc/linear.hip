@@ -13,23 +13,20 @@ namespace {
 // Products over ragged rows: C[i][n] = epi(sum_k A[row(i)][k] B_group[n][k]). PAIR (SwiGLU): a
 // tile's columns are BN / 2 gate columns and their up-projection twins.
 template <typename T, bool BKC, bool PAIR, typename SH>
-__global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(LinearArgs a) {
-  constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN, WAVES = SH::WR * SH::WC;
+__device__ __forceinline__ void rows_tile(const LinearArgs& a, uint4* lds, int tc, int group, int r0, int r1) {
+  constexpr int RT = SH::RT, CT = SH::CT, BM = SH::BM, BN = SH::BN;
   constexpr Map MAP = out_map<T, BKC>();
   constexpr int NCT = PAIR ? CT / 2 : CT;  // tiles of output columns per wave
   constexpr int BW = NCT >= 4 ? 4 : 2;
   static_assert(CT == Slab::CT, "the epilogue's rows");
   typedef Operand<T, BM, true, PLAIN, SH::kThreads> OA;
   typedef Operand<T, BN, BKC, MAP, SH::kThreads> OB;
-  __shared__ uint4 lds[2 * (OA::kChunks + OB::kChunks)];
   uint4 *sA = lds, *sB = lds + 2 * OA::kChunks;
-  static_assert(sizeof(lds) >= WAVES * Slab::kFloats * 4, "the epilogue's rows fit");
+  static_assert(2 * (OA::kChunks + OB::kChunks) * 16 >= SH::WR * SH::WC * Slab::kFloats * 4,
+                "the epilogue's rows fit");
 
   const int f = PAIR ? a.N / 2 : a.N;          // output columns
   constexpr int OBN = PAIR ? BN / 2 : BN;      // output columns of a tile
-  int tr, tc, group, r0, r1;
-  RowTiles<BM> tiles(a);
-  if (!place_tile(tiles.total, (f + OBN - 1) / OBN, tr, tc) || !tiles.find(tr, group, r0, r1)) return;
   const int n0 = tc * OBN;
   const bool none = group >= a.groups;  // rows of no group: zeros
   const int K = none ? 0 : a.K;
@@ -68,11 +65,11 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
 #pragma unroll
     for (int j = 0; j < CT; ++j) acc[i][j] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
   typedef typename Frag<T>::type F;
-  const Reader<T, BM, true, PLAIN, 1> ra(row_w);
-  const Reader<T, BN, BKC, MAP, BW> rb(col_w), ru(OBN + col_w);
+  const Reader<T, BM, true, PLAIN, 1, RT> ra(row_w);
+  const Reader<T, BN, BKC, MAP, BW, NCT> rb(col_w), ru(OBN + col_w);
   auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) {
-    rb.template read<NCT>(lb, s, fb);
-    if constexpr (PAIR) ru.template read<NCT>(lb, s, fb + NCT);
+    rb.read(lb, s, fb);
+    if constexpr (PAIR) ru.read(lb, s, fb + NCT);
   };
   pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, ra, read_b, [](int, const F&, F(&)[CT]) {});
 
@@ -80,6 +77,36 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(Line
   const Slab slab{reinterpret_cast<float*>(lds) + wv * Slab::kFloats};
   const EpilogueBias<T, MAP, PAIR> bias(a, group, none, n0 + col_w, f);
   rows_epilogue<T, MAP, BW, PAIR>(a, acc, slab, bias, none, r0 + row_w, r1, n0 + col_w, f);
+}
+
+// One workgroup a tile. With one workgroup a CU (256 x 256) the tiles that do not fill a whole
+// round of an XCD's 32 CUs would still take one: where they fill no more than half or a quarter
+// of it, each is shared by two or four workgroups, 128 or 64 rows each.
+template <typename T, bool BKC, bool PAIR, typename SH>
+__global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_rows_kernel(LinearArgs a) {
+  constexpr int OBN = PAIR ? SH::BN / 2 : SH::BN;
+  __shared__ uint4 lds[2 * 8 * (SH::BM + SH::BN)];
+  const int tiles_c = ((PAIR ? a.N / 2 : a.N) + OBN - 1) / OBN;
+  int tr, tc, group, r0, r1, parts = 1, part = 0;
+  RowTiles<SH::BM> tiles(a);
+  if constexpr (SH::kShared) {
+    if (!place_shared(tiles.total, tiles_c, tr, tc, part, parts)) return;
+  } else {
+    if (!place_tile(tiles.total, tiles_c, tr, tc)) return;
+  }
+  if (!tiles.find(tr, group, r0, r1)) return;
+  if constexpr (SH::kShared) {
+    if (parts > 1) {
+      r0 += part * (SH::BM / parts);
+      if (r0 >= r1) return;
+      if (parts == 2)
+        rows_tile<T, BKC, PAIR, LinShape<SH::RT / 2, SH::CT, SH::WR, SH::WC, SH::WPS>>(a, lds, tc, group, r0, r1);
+      else
+        rows_tile<T, BKC, PAIR, LinShape<SH::RT / 4, SH::CT, SH::WR, SH::WC, SH::WPS>>(a, lds, tc, group, r0, r1);
+      return;
+    }
+  }
+  rows_tile<T, BKC, PAIR, SH>(a, lds, tc, group, r0, r1);
 }
 
 // Weight gradient: C_group[m][n] = sum over the group's rows r of A[r][m] B[r][n], rows through
@@ -141,9 +168,9 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
   }
 
   typedef typename Frag<T>::type F;
-  const Reader<T, BM, false, MAP, BWR> ra(row_w);
-  const Reader<T, BN, false, MAP, BWC> rb(col_w);
-  auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) { rb.template read<CT>(lb, s, fb); };
+  const Reader<T, BM, false, MAP, BWR, RT> ra(row_w);
+  const Reader<T, BN, false, MAP, BWC, CT> rb(col_w);
+  auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) { rb.read(lb, s, fb); };
   auto extra = [&](int i, const F& fa, F(&fb)[CT]) {
     if constexpr (SIDE == 1) {
       if (sums) sum[i] = mma(ones, fa, sum[i]);
@@ -268,8 +295,16 @@ int launch_rows_shape(LinearArgs& a, hipStream_t s) {
   const int64_t tiles = tiles_r * ((f + obn - 1) / obn);
   a.max_tiles = (int)tiles_r;
   if (tiles > (int64_t)1 << 30) return fail(PULSAR_ERR_INVALID, "linear: launch too large");
-  linear_rows_kernel<T, BKC, PAIR, SH>
-      <<<(unsigned)((tiles + kXcds - 1) / kXcds * kXcds), SH::kThreads, 0, s>>>(a);
+  int64_t slots = (tiles + kXcds - 1) / kXcds;
+  if (SH::kShared) {
+    // shared tiles: of a known number of tiles place_shared's, else up to a round more
+    const int64_t rest = slots % kXcdCus;
+    if (a.offsets)
+      slots += kXcdCus;
+    else
+      slots += rest * (rest * 4 <= kXcdCus ? 3 : rest * 2 <= kXcdCus ? 1 : 0);
+  }
+  linear_rows_kernel<T, BKC, PAIR, SH><<<(unsigned)(slots * kXcds), SH::kThreads, 0, s>>>(a);
   PULSAR_LAUNCH_CHECK();
   return PULSAR_OK;
 }
@@ -290,7 +325,11 @@ double rows_cost(const LinearArgs& a, bool half, int BM, int BN, double rate, do
   if (a.offsets)
     rt = std::max<double>(std::min(a.groups, a.rows), (double)a.rows / BM + 0.6 * a.groups);
   const double n = rt * ((a.N + BN - 1) / BN) / 256;
-  const double rounds = a.offsets ? (n <= 1 ? 1 : n + 0.25) : std::ceil(n);
+  double rounds = a.offsets ? (n <= 1 ? 1 : n + 0.25) : std::ceil(n);
+  if (each > 0) {  // shared tiles: a quarter of a round takes 0.45 of its time, a half 0.65
+    const double rest = n - std::floor(n);
+    rounds = std::floor(n) + (rest == 0 ? 0 : rest <= 0.25 ? 0.45 : rest <= 0.5 ? 0.65 : 1);
+  }
   const double bytes = (double)(BM + BN) * a.K * (half ? 2 : 4), flops = 2.0 * BM * BN * a.K;
   return 4 + rounds * (each + std::max(bytes / rate, flops / flop_rate));
 }
@@ -337,10 +376,7 @@ WgradPlan wgrad_plan(int64_t rows, int64_t groups, int64_t d_in, int64_t d_out, 
     return (int)std::max<int64_t>(1, std::min(fill / std::max<int64_t>(n, 1), rows / groups / 512));
   };
   const int wide = splits(tiles(256), 256);
-#ifndef WGRAD_WIDE
-#define WGRAD_WIDE (groups == 1 && tiles(256) * wide >= 224)
-#endif
-  if (dtype == PULSAR_BF16 && WGRAD_WIDE) return {true, wide};
+  if (dtype == PULSAR_BF16 && groups == 1 && tiles(256) * wide >= 224) return {true, wide};
   return {false, tiles(128) >= 384 ? 1 : splits(tiles(128), 512)};
 }
 

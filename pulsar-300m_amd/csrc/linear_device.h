@@ -38,6 +38,7 @@ struct LinShape {
   static constexpr int RT = RT_, CT = CT_, WR = WR_, WC = WC_, WPS = WPS_;
   static constexpr int kThreads = 64 * WR * WC;
   static constexpr int BM = 16 * RT * WR, BN = 16 * CT * WC;
+  static constexpr bool kShared = kThreads == 512;  // one workgroup a CU
 };
 
 // How a fragment's lane index i (0..15) of tile t maps to the row of the operand's LDS tile.
@@ -52,15 +53,18 @@ enum Map { PLAIN, WIDE, BLOCK };
 //   KC (k contiguous in memory): LDS [R][8] chunks of 16 bytes; chunk c of row r sits at
 //     c ^ key(r), which spreads the 16 rows a fragment read takes over the banks.
 //   otherwise (rows of R contiguous elements per k): LDS [k][R]. bf16 tiles are read through
-//     the LDS transpose load, 4 k rows x 32 bytes per 16 lanes: 32-byte pairs of chunks sit
-//     at pair ^ (k & 3), which puts the 4 rows on different banks. ROWS: k row r is stored row
+//     the LDS transpose load, 4 k rows x 32 bytes per 16 lanes, 32 lanes at once: 32-byte
+//     pairs of chunks sit at pair ^ pair_key(k), which puts those 8 rows (k .. k + 3 and k + 8
+//     .. k + 11) on different banks of the 64. ROWS: k row r is stored row
 //     k_rows[r].
+__device__ __forceinline__ int pair_key(int k) { return (k & 3) | ((k >> 3 & 1) << 2); }
 template <typename T, int R, bool KC, Map MAP, int THREADS, bool ROWS = false>
 struct Operand {
   static constexpr int EV = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T);
   static constexpr int kChunks = R * 8, NCH = kChunks / THREADS;
   static_assert(kChunks % THREADS == 0, "whole chunks per thread");
-  static_assert(KC ? (THREADS / 8) % 16 == 0 : (THREADS * EV / R) % 4 == 0, "one swizzle key per thread");
+  static_assert(KC ? (THREADS / 8) % 16 == 0 : sizeof(T) == 4 || ((THREADS * EV / R) % 16 == 0 && R >= 128),
+                "one swizzle key per thread, eight pairs a row");
 
   const T* base[KC ? NCH : 1];
   int64_t ld;             // !KC: elements from k to k + 1
@@ -94,7 +98,7 @@ struct Operand {
     const int c = (int)threadIdx.x % (R / EV);
     off = (int)threadIdx.x / (R / EV);
     int lc = c;
-    if constexpr (sizeof(T) == 2) lc = (((c >> 1) ^ (off & 3)) << 1) | (c & 1);
+    if constexpr (sizeof(T) == 2) lc = (((c >> 1) ^ pair_key(off)) << 1) | (c & 1);
     int lim;
     const int g = col(lc * EV, lim);
     valid = g < lim;
@@ -155,10 +159,11 @@ struct Frag<float> { typedef lin_f32x4 type; };
 // Reads the fragments of a wave's tiles, whose rows start at row0 of the staged tile: of half s of
 // a step, the lane's 8 bf16 k's 32 s + 8 (lane / 16) .., or its 4 fp32 k's 16 s + 4 (lane / 16) ...
 // The lane's part of the LDS addresses is computed once; tiles and halves differ by constants.
-template <typename T, int R, bool KC, Map MAP, int BW>
+template <typename T, int R, bool KC, Map MAP, int BW, int NT>
 struct Reader {
   static constexpr int kTiles = MAP == BLOCK ? BW : 1;  // of one read_at
-  static constexpr int NV = KC ? 2 : sizeof(T) == 2 ? 4 : 1;
+  static constexpr int NV = KC ? 2 : sizeof(T) == 2 ? NT : 1;
+  static_assert(KC || sizeof(T) == 4 || NT <= 8, "a tile's pair differs from its first's in three bits");
   int off[NV];  // bytes
   __device__ __forceinline__ explicit Reader(int row0) {
     const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
@@ -172,13 +177,12 @@ struct Reader {
       // column j of the 4 rows
       const int k = 8 * kq + (i16 >> 2), c = 4 * (i16 & 3);
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        off[u] = k * (R * 2) + (((row0 >> 4) + u) ^ (k & 3)) * 32 + c * 2;
+      for (int u = 0; u < NT; ++u)
+        off[u] = k * (R * 2) + (((row0 >> 4) + u) ^ pair_key(k)) * 32 + c * 2;
     } else {
       off[0] = (4 * kq * R + row0 + BW * i16) * 4;
     }
   }
-  template <int NT>
   __device__ __forceinline__ void read(const uint4* lds, int s, typename Frag<T>::type* f) const {
 #pragma unroll
     for (int t = 0; t < NT; t += MAP == BLOCK ? BW : 1) read_at(lds, s, t, f + t);
@@ -193,7 +197,7 @@ struct Reader {
     } else if constexpr (sizeof(T) == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4* lds_s4;
-      const char* p = l + off[t & 3] + 32 * s * (R * 2) + (t >> 2) * 128;
+      const char* p = l + off[t] + 32 * s * (R * 2);
       const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
       const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * (R * 2)));
       *f = __builtin_bit_cast(lin_bf16x8,
@@ -378,6 +382,28 @@ __device__ __forceinline__ bool place_tile(int tiles_r, int tiles_c, int& tr, in
   const int per = (total + kXcds - 1) / kXcds, item = xcd * per + slot;
   if (slot >= per || item >= total) return false;
   band_tile(item, kBand, tiles_r, tiles_c, tr, tc);
+  return true;
+}
+
+// The same where the last tiles of an XCD's range, those past whole rounds of its CUs, may be shared:
+// `parts` workgroups a tile.
+constexpr int kXcdCus = 32;
+__device__ __forceinline__ bool place_shared(int tiles_r, int tiles_c, int& tr, int& tc, int& part,
+                                             int& parts) {
+  const int total = tiles_r * tiles_c, xcd = (int)blockIdx.x % kXcds, slot = (int)blockIdx.x / kXcds;
+  const int per = (total + kXcds - 1) / kXcds, first = xcd * per, count = min(per, total - first);
+  if (count <= 0) return false;
+  const int whole = count / kXcdCus * kXcdCus, rest = count - whole;
+  int item = slot;
+  part = 0;
+  parts = 1;
+  if (slot >= whole) {
+    parts = rest * 4 <= kXcdCus ? 4 : rest * 2 <= kXcdCus ? 2 : 1;
+    item = whole + (slot - whole) / parts;
+    part = (slot - whole) % parts;
+  }
+  if (item >= count) return false;
+  band_tile(first + item, kBand, tiles_r, tiles_c, tr, tc);
   return true;
 }
 

@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
   // column of tile t: gate tiles, then their twins
   auto tile_col = [&](int t) { return PAIR && t >= NCT ? a.up + n0 + (t - NCT) * 16 : n0 + t * 16; };
   auto tile_lim = [&](int t) { return PAIR && t >= NCT ? a.up + f : f; };
-  auto kx = [](int k) { return (CT == 2 ? k >> 1 : k) & (CT - 1) & 3; };
+  auto kx = [](int k) { return CT == 1 ? 0 : CT == 2 ? k >> 3 & 1 : (k >> 1 & 1) | (k >> 3 & 1) << 1; };
+  auto kr = [](int k) { return CT == 1 ? k ^ (k >> 3 & 1) << 2 : k; };
   constexpr int NB = BKC ? CT : TR ? CT : MAP == BLOCK ? CT : 1;
   const T* bp[NB];
   bool bn[NB];  // inside the matrix (!BKC)
@@ -87,11 +88,11 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
       bp[t] = Bp + (int64_t)min(tile_col(t) + i16, tile_lim(t) - 1) * a.ldb + kq * EV;
   } else if constexpr (TR) {
     // chunk c of a step: LDS [32 k][CT tiles][2 chunks]; load h covers 32 / CT k rows. A
-    // transposing read takes 32 bytes of 4 k rows at once: tiles sit at t ^ kx(k), which puts
-    // them on different banks
+    // transposing read takes 32 bytes of k rows k .. k + 3 and k + 8 .. k + 11 at once: row k
+    // sits at kr(k) and its tile t at t ^ kx(k), which puts them on different banks of the 64
 #pragma unroll
     for (int h = 0; h < CT; ++h) {
-      const int c = lane + 64 * h, k = c / (2 * CT), t = c / 2 % CT ^ kx(k);
+      const int c = lane + 64 * h, k = kr(c / (2 * CT)), t = c / 2 % CT ^ kx(k);
       const int col = tile_col(t) + 8 * (c & 1);
       bn[h] = col < tile_lim(t);
       bp[h] = Bp + (int64_t)k * a.ldb + (bn[h] ? col : 0);
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
     } else if constexpr (TR) {
 #pragma unroll
       for (int h = 0; h < CT; ++h) {
-        const int k = k0 + (lane + 64 * h) / (2 * CT);
+        const int k = k0 + kr((lane + 64 * h) / (2 * CT));
         w[h] = load_chunk(bp[h] + (int64_t)k0 * a.ldb, s < s1 && k < kend && bn[h]);
       }
     } else {
@@ -174,10 +175,12 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
         for (int h = 0; h < CT; ++h) stage[lane + 64 * h] = wbuf[d][h];
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-          const char* p = reinterpret_cast<const char*>(stage) +
-                          (8 * kq + (i16 >> 2)) * (CT * 32) + (t ^ kx(i16 >> 2)) * 32 + (i16 & 3) * 8;
-          const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
-          const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * CT * 32));
+          const int k = 8 * kq + (i16 >> 2);
+          auto at = [&](int r) {
+            return reinterpret_cast<const char*>(stage) + kr(r) * (CT * 32) + (t ^ kx(r)) * 32 + (i16 & 3) * 8;
+          };
+          const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at(k));
+          const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at(k + 4));
           fb[t] = __builtin_bit_cast(F, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
       } else {
