@@ -60,18 +60,33 @@ __device__ __forceinline__ void rows_tile(const LinearArgs& a, uint4* lds, int t
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int row_w = wv / SH::WC * RT * 16, col_w = wv % SH::WC * NCT * 16;
   lin_f32x4 acc[RT][CT];
+  clear(acc);
+  bool again = true;  // fp32: the split products, and the plain ones where they were not finite
+  if constexpr (sizeof(T) == 4) {
+    const SplitReader<BM, true, 1> ra(row_w);
+    const SplitReader<BN, BKC, BW> rb(col_w), ru(OBN + col_w);
+    auto read_b = [&](const uint4* lb, float(&x)[CT][8]) {
+      constexpr int BT = decltype(rb)::kTiles;
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < CT; ++j) acc[i][j] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
-  typedef typename Frag<T>::type F;
-  const Reader<T, BM, true, PLAIN, 1, RT> ra(row_w);
-  const Reader<T, BN, BKC, MAP, BW, NCT> rb(col_w), ru(OBN + col_w);
-  auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) {
-    rb.read(lb, s, fb);
-    if constexpr (PAIR) ru.read(lb, s, fb + NCT);
-  };
-  pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, ra, read_b, [](int, const F&, F(&)[CT]) {});
+      for (int j = 0; j < NCT; j += BT) {
+        rb.read(lb, j, x + j);
+        if constexpr (PAIR) ru.read(lb, j, x + NCT + j);
+      }
+    };
+    split_loop<SH>(oa, ob, K, sA, sB, acc, ra, read_b, [](int, const Split&, Split(&)[CT]) {});
+    again = any_not_finite(acc);
+    if (again) clear(acc);
+  }
+  if (again) {
+    typedef typename Frag<T>::type F;
+    const Reader<T, BM, true, PLAIN, 1, RT> ra(row_w);
+    const Reader<T, BN, BKC, MAP, BW, NCT> rb(col_w), ru(OBN + col_w);
+    auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) {
+      rb.read(lb, s, fb);
+      if constexpr (PAIR) ru.read(lb, s, fb + NCT);
+    };
+    pipe_loop<T, SH>(oa, ob, K, sA, sB, acc, ra, read_b, [](int, const F&, F(&)[CT]) {});
+  }
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   const Slab slab{reinterpret_cast<float*>(lds) + wv * Slab::kFloats};
@@ -153,39 +168,62 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
   const int wr = wv / SH::WC, wc = wv % SH::WC;
   const int i16 = lane & 15, kq = lane >> 4;
   const int row_w = wr * RT * 16, col_w = wc * CT * 16;
-  lin_f32x4 acc[RT][CT], sum[SIDE == 1 ? RT : CT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < CT; ++j) acc[i][j] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
-  typename Frag<T>::type ones;
-#pragma unroll
-  for (int e = 0; e < OA::EV; ++e) ones[e] = 1.f;
+  lin_f32x4 acc[RT][CT], sum[1][SIDE == 1 ? RT : CT];
+  clear(acc);
+  clear(sum);
   const bool sums = SIDE == 1 ? tc == 0 && wc == 0 : SIDE == 2 ? mt == 0 && wr == 0 : false;
-  if constexpr (SIDE != 0) {
+  bool again = true;
+  if constexpr (sizeof(T) == 4) {
+    const SplitReader<BM, false, BWR> ra(row_w);
+    const SplitReader<BN, false, BWC> rb(col_w);
+    auto read_b = [&](const uint4* lb, float(&x)[CT][8]) {
 #pragma unroll
-    for (int i = 0; i < (SIDE == 1 ? RT : CT); ++i) sum[i] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < CT; j += BWC) rb.read(lb, j, x + j);
+    };
+    lin_bf16x8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = 1.f;
+    auto extra = [&](int i, const Split& fa, Split(&fb)[CT]) {
+      if constexpr (SIDE == 1) {
+        if (sums) sum[0][i] = mma(ones, fa.h, mma(ones, fa.m, mma(ones, fa.l, sum[0][i])));
+      }
+      if constexpr (SIDE == 2) {
+        if (sums && i == 0)
+#pragma unroll
+          for (int j = 0; j < CT; ++j) sum[0][j] = mma(fb[j].h, ones, mma(fb[j].m, ones, mma(fb[j].l, ones, sum[0][j])));
+      }
+    };
+    split_loop<SH>(oa, ob, r1 - r0, sA, sB, acc, ra, read_b, extra);
+    again = any_not_finite(acc) || (SIDE != 0 && any_not_finite(sum));
+    if (again) {
+      clear(acc);
+      clear(sum);
+    }
   }
-
-  typedef typename Frag<T>::type F;
-  const Reader<T, BM, false, MAP, BWR, RT> ra(row_w);
-  const Reader<T, BN, false, MAP, BWC, CT> rb(col_w);
-  auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) { rb.read(lb, s, fb); };
-  auto extra = [&](int i, const F& fa, F(&fb)[CT]) {
-    if constexpr (SIDE == 1) {
-      if (sums) sum[i] = mma(ones, fa, sum[i]);
-    }
-    if constexpr (SIDE == 2) {
-      if (sums && i == 0)
+  if (again) {
+    typedef typename Frag<T>::type F;
+    F ones;
 #pragma unroll
-        for (int j = 0; j < CT; ++j) sum[j] = mma(fb[j], ones, sum[j]);
-    }
-  };
-  pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, ra, read_b, extra);
+    for (int e = 0; e < OA::EV; ++e) ones[e] = 1.f;
+    const Reader<T, BM, false, MAP, BWR, RT> ra(row_w);
+    const Reader<T, BN, false, MAP, BWC, CT> rb(col_w);
+    auto read_b = [&](const uint4* lb, int s, F(&fb)[CT]) { rb.read(lb, s, fb); };
+    auto extra = [&](int i, const F& fa, F(&fb)[CT]) {
+      if constexpr (SIDE == 1) {
+        if (sums) sum[0][i] = mma(ones, fa, sum[0][i]);
+      }
+      if constexpr (SIDE == 2) {
+        if (sums && i == 0)
+#pragma unroll
+          for (int j = 0; j < CT; ++j) sum[0][j] = mma(fb[j], ones, sum[0][j]);
+      }
+    };
+    pipe_loop<T, SH>(oa, ob, r1 - r0, sA, sB, acc, ra, read_b, extra);
+  }
 
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   const Slab slab{reinterpret_cast<float*>(lds) + wv * Slab::kFloats};
-  wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum, slab, sums, group, split, m0 + row_w, n0 + col_w);
+  wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum[0], slab, sums, group, split, m0 + row_w, n0 + col_w);
 }
 
 // Sums of a weight gradient's splits, in order; `count` elements of one split's partials, the
@@ -312,8 +350,9 @@ int launch_rows_shape(LinearArgs& a, hipStream_t s) {
 // Expected us of a product in tiles of BM x BN, by what bounds them here: each CU streams the
 // operands of its tiles from the caches at `rate` bytes/us (35 KB/us for the few-row kernels,
 // 45-49 for the tile kernels with two workgroups a CU, 38 for 256 x 256, whose tiles also pay
-// `each` us of start and end that nothing overlaps) or multiplies at 5 (bf16) or 0.5 (fp32)
-// MFLOP/us, whichever takes longer, after about 4 us of launch and first loads. Measured against
+// `each` us of start and end that nothing overlaps) or multiplies at flop_rate (5 MFLOP/us in
+// bf16; in fp32 0.25 - 0.33 in the few-row kernels, 0.5 - 0.6 in the tiles), whichever takes
+// longer, after about 4 us of launch and first loads. Measured against
 // it, us (model): 16 rows x 1024 x 1024 in 16 x 16 tiles 5.7 (5.8), in 16 x 32 6.3 (6.7); 512
 // rows 32 x 64 9.7 (9.5), 32 x 32 12.0 (11.3), 64 x 64 12.4 (11.3); 4096 columns x 4096 k, 64
 // rows in 32 x 32 19.7 (18.6), 32 x 64 26 (25.9); 2048 rows in 64 x 128 12.6 (12.5); 16384 x 2048
@@ -347,8 +386,8 @@ int launch_rows(LinearArgs& a, bool b_kc, hipStream_t s) {
   for (int i = pair ? 1 : 0; i < 6; ++i)
     offer(i, rows_cost(a, half, 16 * kFewShapes[i].rt, 16 * kFewShapes[i].ct, 35e3,
                        half ? 5e6 : b_kc ? 0.33e6 : 0.25e6, 0));
-  offer(6, rows_cost(a, half, 64, 128, 45e3, half ? 5e6 : 0.47e6, 0));
-  offer(7, rows_cost(a, half, 128, 128, 49e3, half ? 5e6 : 0.5e6, 0));
+  offer(6, rows_cost(a, half, 64, 128, 45e3, half ? 5e6 : 0.5e6, 0));
+  offer(7, rows_cost(a, half, 128, 128, 49e3, half ? 5e6 : 0.6e6, 0));
   if (half) offer(8, rows_cost(a, half, 256, 256, 38e3, 5e6, 10));
   if (best < 6) return launch_linear_few(a, half ? PULSAR_BF16 : PULSAR_F32, b_kc, best, s);
   auto go = [&](auto kc, auto pr) {

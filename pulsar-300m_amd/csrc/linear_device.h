@@ -229,6 +229,151 @@ __device__ __forceinline__ lin_f32x4 mma(lin_f32x4 a, lin_f32x4 b, lin_f32x4 c) 
   return c;
 }
 
+// fp32 products on the bf16 matrix cores, which are 16 times as fast as the fp32 ones: x = h + m + l
+// exactly, 8 significant bits each by rounding to the nearest, and a b = the six products down
+// to m m and h l. What is left out, m l, l m and l l, is at most 2^-24 of |a b| (|m| <= 2^-8,
+// |l| <= 2^-17 of the largest power of two in |x|), half a step of fp32. Each kept product is
+// exact in fp32 and summed in fp32. An infinite x, or one that rounds to infinity, gives m = NaN:
+// results that are not finite are computed again by the fp32 products. (Below 2^-110 l is a
+// subnormal bf16.)
+struct Split {
+  lin_bf16x8 h, m, l;
+  __device__ __forceinline__ explicit Split(const float (&x)[8]) {
+    // two values an instruction where there is one
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    auto round2 = [](f2 v) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2)); };
+    auto rest = [](f2 v, uint32_t r) {
+      return f2{v[0] - __uint_as_float(r << 16), v[1] - __uint_as_float(r & 0xffff0000u)};
+    };
+    uint32_t w[3][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f2 v = {x[2 * q], x[2 * q + 1]};
+      w[0][q] = round2(v);
+      const f2 r = rest(v, w[0][q]);
+      w[1][q] = round2(r);
+      w[2][q] = round2(rest(r, w[1][q]));
+    }
+    __builtin_memcpy(&h, w[0], 16);
+    __builtin_memcpy(&m, w[1], 16);
+    __builtin_memcpy(&l, w[2], 16);
+  }
+};
+__device__ __forceinline__ lin_f32x4 mma(const Split& a, const Split& b, lin_f32x4 c) {
+  c = mma(a.l, b.h, c);
+  c = mma(a.h, b.l, c);
+  c = mma(a.m, b.m, c);
+  c = mma(a.m, b.h, c);
+  c = mma(a.h, b.m, c);
+  return mma(a.h, b.h, c);
+}
+
+// Reads a wave's fp32 tiles for them: the lane's 8 k's 8 (lane / 16) .. of a whole step.
+template <int R, bool KC, int BW>
+struct SplitReader {
+  static constexpr int kTiles = KC ? 1 : BW;
+  int off[2];  // bytes
+  __device__ __forceinline__ explicit SplitReader(int row0) {
+    const int lane = (int)threadIdx.x & 63, i16 = lane & 15, kq = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      off[s] = KC ? (row0 + i16) * 128 + ((2 * kq + s) ^ (i16 & 7)) * 16 : (8 * kq * R + row0 + BW * i16) * 4;
+  }
+  // Tile t (!KC: the BW tiles from it).
+  __device__ __forceinline__ void read(const uint4* lds, int t, float (*f)[8]) const {
+    const char* l = reinterpret_cast<const char*>(lds);
+    if constexpr (KC) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        *reinterpret_cast<lin_f32x4*>(&f[0][4 * s]) = *reinterpret_cast<const lin_f32x4*>(l + off[s] + t * 2048);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float* p = reinterpret_cast<const float*>(l + off[0] + (j * R + 16 * t) * 4);
+        float v[BW];
+        __builtin_memcpy(v, __builtin_assume_aligned(p, 4 * BW), sizeof(v));
+#pragma unroll
+        for (int b = 0; b < BW; ++b) f[b][j] = v[b];
+      }
+    }
+  }
+};
+
+// Their main loop. A step's values wait in registers: while they are split and multiplied, the next
+// step's are read over them from the other LDS buffer, and the step after next is loaded into
+// the buffer they came from. extra(i, a, b) as pipe_loop's.
+template <typename SH, typename OA, typename OB, typename RA, typename RB, typename EX>
+__device__ __forceinline__ void split_loop(OA& oa, OB& ob, int K, uint4* sA, uint4* sB,
+                                           lin_f32x4 (&acc)[SH::RT][SH::CT], const RA& ra, RB&& rb,
+                                           EX&& extra) {
+  constexpr int RT = SH::RT, CT = SH::CT, BK = OA::BK, LA = OA::NCH, LB = OB::NCH, AT = RA::kTiles;
+  const int steps = (K + BK - 1) / BK;
+  if (steps == 0) return;
+  const uint32_t da = lds_address(sA), db = lds_address(sB);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    oa.prefetch(p * BK, K);
+    ob.prefetch(p * BK, K);
+#pragma unroll
+    for (int c = 0; c < LA; ++c) oa.fetch(c, p * BK, K, da + p * OA::kChunks * 16);
+#pragma unroll
+    for (int c = 0; c < LB; ++c) ob.fetch(c, p * BK, K, db + p * OB::kChunks * 16);
+  }
+  oa.prefetch(2 * BK, K);
+  ob.prefetch(2 * BK, K);
+  wait_vmcnt<LA + LB>();
+  lds_barrier();
+  float xa[RT][8], xb[CT][8];
+  rb(sB, xb);
+#pragma unroll
+  for (int i = 0; i < RT; i += AT) ra.read(sA, i, xa + i);
+#pragma unroll 1
+  for (int st = 0; st < steps; ++st) {
+    const int x = st & 1, y = x ^ 1, k0 = (st + 2) * BK;
+    wait_vmcnt<0>();
+    lds_barrier();  // step st is in registers everywhere, step st + 1 in buffer y
+    static_assert(CT == 4, "as many as there are initialisers");
+    Split b[CT] = {Split(xb[0]), Split(xb[1]), Split(xb[2]), Split(xb[3])};
+    rb(sB + y * OB::kChunks, xb);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const Split a(xa[i]);
+      if (i % AT == AT - 1) ra.read(sA + y * OA::kChunks, i - (AT - 1), xa + i - (AT - 1));
+#pragma unroll
+      for (int c = i * LA / RT; c < (i + 1) * LA / RT; ++c) oa.fetch(c, k0, K, da + x * (OA::kChunks * 16));
+#pragma unroll
+      for (int c = i * LB / RT; c < (i + 1) * LB / RT; ++c) ob.fetch(c, k0, K, db + x * (OB::kChunks * 16));
+#pragma unroll
+      for (int j = 0; j < CT; ++j) acc[i][j] = mma(b[j], a, acc[i][j]);
+      extra(i, a, b);
+    }
+    oa.prefetch(k0 + BK, K);
+    ob.prefetch(k0 + BK, K);
+  }
+  wait_vmcnt<0>();  // the loads past the end: their buffers are used again
+}
+
+// Whether any of the workgroup's sums is not finite.
+template <int RT, int CT>
+__device__ __forceinline__ bool any_not_finite(const lin_f32x4 (&acc)[RT][CT]) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = fmaf(acc[i][j][e], 0.f, s);
+  return __syncthreads_or(s != s);
+}
+template <int N, int M>
+__device__ __forceinline__ void clear(lin_f32x4 (&acc)[N][M]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < M; ++j) acc[i][j] = lin_f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 // The main loop: acc += A tile . B tile^T over K, B as the matrix core's first operand, so that a
 // lane ends with 4 consecutive n of its own m.
 //

@@ -1,6 +1,7 @@
 // Native half of the pulsar_cuda op surface: output allocation, the current stream and the
 // library call of each op, for the Python wrappers in pulsar_cuda/__init__.py, which have
-// checked the operands (device, dtype, shape, contiguity) before they come here.
+// checked the operands (device, dtype, shape, contiguity) before they come here; the linear ops'
+// operands are checked here.
 //
 // A call through ctypes with its outputs from torch.empty costs 5 us of Python beside the
 // 3.4 us of the launch itself (output tensors 2.6, torch.cuda.current_stream 2.0, argument
@@ -368,101 +369,213 @@ Tensor workspace(const Tensor& on, int64_t bytes) {
 }
 void* wp(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// The checks of the linear ops are here, not in Python, where they took 3 us of an 8 us call. Types
+// and shapes first, the device last, before anything is allocated or launched.
+void on_device(const Tensor& t, const char* name, const Tensor& x) {
+  TORCH_CHECK(t.device() == x.device(), name, " must be on the device of x");
+}
+void float_type(const Tensor& x) {
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat,
+              "x must be bfloat16 or float32, got ", x.scalar_type());
+}
+void same_type(const Tensor& t, const char* name, const Tensor& x) {
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must have the dtype of x");
+}
+void on_gpu(const Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+}
+void shaped(const Tensor& t, const char* name, at::IntArrayRef shape) {
+  TORCH_CHECK(t.sizes() == shape, name, " must be ", shape, ", got ", t.sizes());
+}
+int64_t out_cols(int64_t act, int64_t d_out) {
+  if (act != PULSAR_ACT_SWIGLU) return d_out;
+  TORCH_CHECK(d_out % 2 == 0, "swiglu needs an even number of output columns, got ", d_out);
+  return d_out / 2;
+}
+// An optional bias, of x's type or fp32.
+Tensor checked_bias(const Tensor& b, const Tensor& x, at::IntArrayRef shape) {
+  if (!b.defined()) return b;
+  TORCH_CHECK(b.scalar_type() == x.scalar_type() || b.scalar_type() == at::kFloat,
+              "bias must have the dtype of x or be float32");
+  shaped(b, "bias", shape);
+  on_device(b, "bias", x);
+  return b.contiguous();
+}
+Tensor checked_index(const Tensor& t, const char* name, const Tensor& x) {
+  if (!t.defined()) return t;
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1, name, " must be 1-dimensional int32");
+  on_device(t, name, x);
+  return t.contiguous();
+}
+// The pre-activation values of a backward call that needs them.
+Tensor checked_pre(const Tensor& pre, int64_t act, const Tensor& x, at::IntArrayRef shape) {
+  if (act == PULSAR_ACT_NONE) return Tensor();
+  TORCH_CHECK(pre.defined(), "pre is needed for every activation but none");
+  same_type(pre, "pre", x);
+  shaped(pre, "pre", shape);
+  on_device(pre, "pre", x);
+  return pre.contiguous();
+}
+std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = n;
+  return shape;
+}
+
 // (topk_idx, E) -> (offsets, rows, slots)
 PyObject* moe_group_rows(const Args& a) {
-  const Tensor& idx = a.t(0);
-  const int64_t N = idx.size(0), K = idx.size(1), E = a.i64(1);
+  const Tensor& t = a.t(0);
+  const int64_t E = a.i64(1);
+  TORCH_CHECK(t.scalar_type() == at::kLong, "topk_idx must be int64");
+  TORCH_CHECK(t.dim() == 2 && t.size(1) > 0, "topk_idx must be [N, K]");
+  TORCH_CHECK(E > 0 && E <= 1024, "moe_group_rows supports 1 <= E <= 1024, got ", E);
+  on_gpu(t, "topk_idx");
+  const Tensor idx = t.contiguous();
+  const int64_t N = idx.size(0), K = idx.size(1);
   const c10::DeviceGuard guard(idx.device());
-  const int64_t bytes = pulsar_moe_group_rows_workspace_bytes(N, K, E);
+  const Tensor ws = workspace(idx, pulsar_moe_group_rows_workspace_bytes(N, K, E));
   Tensor o = make(idx, {E + 1}, at::kInt), r = make(idx, {N * K}, at::kInt);
-  Tensor s = make(idx, {N, K}, at::kInt), ws;
-  if (bytes > 0) ws = make(idx, {bytes / 4}, at::kInt);
+  Tensor s = make(idx, {N, K}, at::kInt);
   run(pulsar_moe_group_rows, p<int64_t>(idx), q<int32_t>(o), q<int32_t>(r), q<int32_t>(s), N, K, E,
       wp(ws), stream(idx));
   return triple(o, r, s, false);
 }
 
+struct Linear {  // operands of the dense ops
+  const Tensor &x, &w;
+  int64_t act, I, O, cols, rows, so, si, xs;
+  Linear(const Tensor& x_, const Tensor& w_, int64_t act_) : x(x_), w(w_), act(act_) {
+    float_type(x);
+    same_type(w, "weight", x);
+    TORCH_CHECK(w.dim() == 2, "weight must be [d_out, d_in]");
+    O = w.size(0);
+    I = w.size(1);
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) == I, "x must be [..., d_in]");
+    TORCH_CHECK(O > 0 && I > 0, "weight must not be empty");
+    cols = out_cols(act, O);
+    rows = x.numel() / I;
+    weight_strides(w, so, si);
+    xs = row_stride(x, "x");
+  }
+  void device() const {
+    on_gpu(x, "x");
+    on_device(w, "weight", x);
+  }
+};
+
 // (x, weight [O, I], bias, residual, activation, save_pre) -> y or (y, pre)
 PyObject* fused_linear_forward(const Args& a) {
-  const Tensor &x = a.t(0), &w = a.t(1);
-  const Tensor b = a.opt(2), res = a.opt(3);
-  const int64_t act = a.i64(4), I = x.size(-1), O = w.size(0), rows = x.numel() / I;
-  int64_t so, si;
-  weight_strides(w, so, si);
-  const int64_t xs = row_stride(x, "x"), rs = res.defined() ? row_stride(res, "residual") : 0;
-  const c10::DeviceGuard guard(x.device());
-  std::vector<int64_t> shape = x.sizes().vec();
+  const Linear l(a.t(0), a.t(1), a.i64(4));
+  const Tensor b = checked_bias(a.opt(2), l.x, {l.O}), res = a.opt(3);
+  int64_t rs = 0;
+  if (res.defined()) {
+    same_type(res, "residual", l.x);
+    shaped(res, "residual", with_last(l.x, l.cols));
+    on_device(res, "residual", l.x);
+    rs = row_stride(res, "residual");
+  }
+  l.device();
+  const c10::DeviceGuard guard(l.x.device());
   Tensor pre;
-  shape.back() = O;
-  if (a.i64(5)) pre = make(x, shape);
-  if (act == PULSAR_ACT_SWIGLU) shape.back() = O / 2;
-  Tensor y = make(x, shape);
-  const Tensor ws = workspace(x, pulsar_fused_linear_forward_workspace_bytes(
-      x.data_ptr(), xs, w.data_ptr(), so, si, rows, I, O, (int)act, code(x)));
-  run(pulsar_fused_linear_forward, p(x), xs, p(w), so, si, p(b), b.defined() ? code(b) : 0, p(res),
-      rs, q(y), pre.defined() ? q(pre) : nullptr, rows, I, O, (int)act, code(x), wp(ws),
-      stream(x));
+  if (a.i64(5)) pre = make(l.x, with_last(l.x, l.O));
+  Tensor y = make(l.x, with_last(l.x, l.cols));
+  const Tensor ws = workspace(l.x, pulsar_fused_linear_forward_workspace_bytes(
+      l.x.data_ptr(), l.xs, l.w.data_ptr(), l.so, l.si, l.rows, l.I, l.O, (int)l.act, code(l.x)));
+  run(pulsar_fused_linear_forward, p(l.x), l.xs, p(l.w), l.so, l.si, p(b), b.defined() ? code(b) : 0,
+      p(res), rs, q(y), pre.defined() ? q(pre) : nullptr, l.rows, l.I, l.O, (int)l.act, code(l.x),
+      wp(ws), stream(l.x));
   return pre.defined() ? pair(y, pre, false) : out(y);
 }
 
 // (dy, x, weight [O, I], pre, activation, bias) -> [dx, dw, db]
 PyObject* fused_linear_backward(const Args& a) {
-  const Tensor &dy = a.t(0), &x = a.t(1), &w = a.t(2);
-  const Tensor pre = a.opt(3);
-  const int64_t act = a.i64(4), I = x.size(-1), O = w.size(0), rows = x.numel() / I;
-  int64_t so, si;
-  weight_strides(w, so, si);
-  const int64_t xs = row_stride(x, "x");
-  const c10::DeviceGuard guard(x.device());
-  Tensor dx = make(x, x.sizes()), dw = weight_grad(w, si == 1), db;
-  if (a.i64(5)) db = make(x, {O});
-  const Tensor ws = workspace(x, pulsar_fused_linear_backward_workspace_bytes(
-      dy.data_ptr(), x.data_ptr(), xs, w.data_ptr(), so, si, rows, I, O, (int)act, code(x)));
-  run(pulsar_fused_linear_backward, p(dy), p(x), xs, p(w), so, si, p(pre), q(dx), q(dw),
-      db.defined() ? q(db) : nullptr, rows, I, O, (int)act, code(x), wp(ws), stream(x));
+  const Linear l(a.t(1), a.t(2), a.i64(4));
+  const Tensor& d = a.t(0);
+  same_type(d, "dy", l.x);
+  shaped(d, "dy", with_last(l.x, l.cols));
+  on_device(d, "dy", l.x);
+  const Tensor pre = checked_pre(a.opt(3), l.act, l.x, with_last(l.x, l.O));
+  l.device();
+  const c10::DeviceGuard guard(l.x.device());
+  const Tensor dy = d.contiguous();
+  Tensor dx = make(l.x, l.x.sizes()), dw = weight_grad(l.w, l.si == 1), db;
+  if (a.i64(5)) db = make(l.x, {l.O});
+  const Tensor ws = workspace(l.x, pulsar_fused_linear_backward_workspace_bytes(
+      dy.data_ptr(), l.x.data_ptr(), l.xs, l.w.data_ptr(), l.so, l.si, l.rows, l.I, l.O, (int)l.act,
+      code(l.x)));
+  run(pulsar_fused_linear_backward, p(dy), p(l.x), l.xs, p(l.w), l.so, l.si, p(pre), q(dx), q(dw),
+      db.defined() ? q(db) : nullptr, l.rows, l.I, l.O, (int)l.act, code(l.x), wp(ws), stream(l.x));
   return triple(dx, dw, db, true);
 }
 
+struct Grouped {  // operands of the ragged ops
+  const Tensor &x, &w;
+  Tensor off, idx;
+  int64_t act, E, I, O, cols, M, si, so, xs;
+  Grouped(const Tensor& x_, const Tensor& w_, const Tensor& off_, const Tensor& idx_, int64_t act_)
+      : x(x_), w(w_), act(act_) {
+    float_type(x);
+    same_type(w, "weight", x);
+    TORCH_CHECK(w.dim() == 3, "weight must be [E, d_in, d_out]");
+    E = w.size(0);
+    I = w.size(1);
+    O = w.size(2);
+    TORCH_CHECK(x.dim() == 2 && x.size(1) == I, "x must be [R, d_in]");
+    TORCH_CHECK(E > 0 && I > 0 && O > 0, "weight must not be empty");
+    cols = out_cols(act, O);
+    off = checked_index(off_, "offsets", x);
+    TORCH_CHECK(off.numel() == E + 1, "offsets must have E + 1 elements");
+    idx = checked_index(idx_, "rows", x);
+    M = idx.defined() ? idx.numel() : x.size(0);
+    weight_strides(w, si, so);
+    xs = row_stride(x, "x");
+  }
+  void device() const {
+    on_gpu(x, "x");
+    on_device(w, "weight", x);
+  }
+};
+
 // (x, weight [E, I, O], offsets, rows, bias, activation, save_pre) -> y or (y, pre)
 PyObject* grouped_linear_forward(const Args& a) {
-  const Tensor &x = a.t(0), &w = a.t(1), &off = a.t(2);
-  const Tensor idx = a.opt(3), b = a.opt(4);
-  const int64_t act = a.i64(5), E = w.size(0), I = w.size(1), O = w.size(2);
-  const int64_t M = idx.defined() ? idx.numel() : x.size(0);
-  int64_t si, so;
-  weight_strides(w, si, so);
-  const int64_t xs = row_stride(x, "x");
-  const c10::DeviceGuard guard(x.device());
+  const Grouped l(a.t(0), a.t(1), a.t(2), a.opt(3), a.i64(5));
+  const Tensor b = checked_bias(a.opt(4), l.x, {l.E, l.O});
+  l.device();
+  const c10::DeviceGuard guard(l.x.device());
   Tensor pre;
-  if (a.i64(6)) pre = make(x, {M, O});
-  Tensor y = make(x, {M, act == PULSAR_ACT_SWIGLU ? O / 2 : O});
-  const Tensor ws = workspace(x, pulsar_grouped_linear_forward_workspace_bytes(
-      x.data_ptr(), xs, x.size(0), w.data_ptr(), w.stride(0), si, so, M, E, I, O, (int)act, code(x)));
-  run(pulsar_grouped_linear_forward, p(x), xs, x.size(0), p<int32_t>(idx), p<int32_t>(off), p(w),
-      w.stride(0), si, so, p(b), b.defined() ? code(b) : 0, q(y),
-      pre.defined() ? q(pre) : nullptr, M, E, I, O, (int)act, code(x), wp(ws),
-      stream(x));
+  if (a.i64(6)) pre = make(l.x, {l.M, l.O});
+  Tensor y = make(l.x, {l.M, l.cols});
+  const Tensor ws = workspace(l.x, pulsar_grouped_linear_forward_workspace_bytes(
+      l.x.data_ptr(), l.xs, l.x.size(0), l.w.data_ptr(), l.w.stride(0), l.si, l.so, l.M, l.E, l.I,
+      l.O, (int)l.act, code(l.x)));
+  run(pulsar_grouped_linear_forward, p(l.x), l.xs, l.x.size(0), p<int32_t>(l.idx),
+      p<int32_t>(l.off), p(l.w), l.w.stride(0), l.si, l.so, p(b), b.defined() ? code(b) : 0, q(y),
+      pre.defined() ? q(pre) : nullptr, l.M, l.E, l.I, l.O, (int)l.act, code(l.x), wp(ws),
+      stream(l.x));
   return pre.defined() ? pair(y, pre, false) : out(y);
 }
 
 // (dy, x, weight [E, I, O], offsets, rows, pre, activation, bias) -> [dx, dw, db]
 PyObject* grouped_linear_backward(const Args& a) {
-  const Tensor &dy = a.t(0), &x = a.t(1), &w = a.t(2), &off = a.t(3);
-  const Tensor idx = a.opt(4), pre = a.opt(5);
-  const int64_t act = a.i64(6), E = w.size(0), I = w.size(1), O = w.size(2), M = dy.size(0);
-  int64_t si, so;
-  weight_strides(w, si, so);
-  const int64_t xs = row_stride(x, "x");
-  const c10::DeviceGuard guard(x.device());
+  const Grouped l(a.t(1), a.t(2), a.t(3), a.opt(4), a.i64(6));
+  const Tensor& d = a.t(0);
+  same_type(d, "dy", l.x);
+  shaped(d, "dy", {l.M, l.cols});
+  on_device(d, "dy", l.x);
+  const Tensor pre = checked_pre(a.opt(5), l.act, l.x, {l.M, l.O});
+  l.device();
+  const c10::DeviceGuard guard(l.x.device());
+  const Tensor dy = d.contiguous();
   // the library writes dw with the input dimension contiguous where the weight's is
-  Tensor dx = make(x, {M, I}), dw = weight_grad(w, si != 1), db;
-  if (a.i64(7)) db = make(x, {E, O});
-  const Tensor ws = workspace(x, pulsar_grouped_linear_backward_workspace_bytes(
-      dy.data_ptr(), x.data_ptr(), xs, x.size(0), w.data_ptr(), w.stride(0), si, so, M, E, I, O,
-      (int)act, code(x)));
-  run(pulsar_grouped_linear_backward, p(dy), p(x), xs, x.size(0), p<int32_t>(idx), p<int32_t>(off),
-      p(w), w.stride(0), si, so, p(pre), q(dx), q(dw), db.defined() ? q(db) : nullptr, M, E, I, O,
-      (int)act, code(x), wp(ws), stream(x));
+  Tensor dx = make(l.x, {l.M, l.I}), dw = weight_grad(l.w, l.si != 1), db;
+  if (a.i64(7)) db = make(l.x, {l.E, l.O});
+  const Tensor ws = workspace(l.x, pulsar_grouped_linear_backward_workspace_bytes(
+      dy.data_ptr(), l.x.data_ptr(), l.xs, l.x.size(0), l.w.data_ptr(), l.w.stride(0), l.si, l.so,
+      l.M, l.E, l.I, l.O, (int)l.act, code(l.x)));
+  run(pulsar_grouped_linear_backward, p(dy), p(l.x), l.xs, l.x.size(0), p<int32_t>(l.idx),
+      p<int32_t>(l.off), p(l.w), l.w.stride(0), l.si, l.so, p(pre), q(dx), q(dw),
+      db.defined() ? q(db) : nullptr, l.M, l.E, l.I, l.O, (int)l.act, code(l.x), wp(ws),
+      stream(l.x));
   return triple(dx, dw, db, true);
 }
 

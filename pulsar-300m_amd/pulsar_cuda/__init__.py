@@ -425,37 +425,14 @@ def moe_combine_backward(d_routed_out: torch.Tensor, expert_outputs: torch.Tenso
 # Products with their epilogues, dense and ragged
 # ---------------------------------------------------------------------------
 
-def _act_code(activation: str, d_out: int) -> int:
+# The native half checks these operands (types, shapes, strides, devices): the checks in Python cost
+# as much as the launch of a decoding step's product.
+
+def _act_code(activation: str) -> int:
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    if activation == "swiglu" and d_out % 2:
-        raise RuntimeError(f"swiglu needs an even number of output columns, got {d_out}")
     return code
-
-
-def _operand(t: torch.Tensor, name: str, x: torch.Tensor) -> None:
-    """A tensor of x's dtype on x's device."""
-    _cuda(t, name)
-    _req(t.device == x.device, f"{name} must be on the device of x")
-    _req(t.dtype == x.dtype, f"{name} must have the dtype of x")
-
-
-def _bias(bias, x: torch.Tensor, shape: tuple):
-    if bias is None:
-        return None
-    _cuda(bias, "bias")
-    _req(bias.device == x.device, "bias must be on the device of x")
-    _req(bias.dtype in (x.dtype, torch.float32), "bias must have the dtype of x or be float32")
-    _req(tuple(bias.shape) == shape, f"bias must be {list(shape)}, got {list(bias.shape)}")
-    return bias.contiguous()
-
-
-def _index(t: torch.Tensor, name: str, x: torch.Tensor) -> torch.Tensor:
-    _cuda(t, name)
-    _req(t.device == x.device, f"{name} must be on the device of x")
-    _req(t.dtype == torch.int32 and t.dim() == 1, f"{name} must be 1-dimensional int32")
-    return t.contiguous()
 
 
 def moe_group_rows(topk_idx: torch.Tensor, num_experts: int):
@@ -468,21 +445,7 @@ def moe_group_rows(topk_idx: torch.Tensor, num_experts: int):
 
     The combine of the rows takes the slots as they are, all rows as one expert's:
     ``moe_combine_forward(y[None], torch.zeros_like(topk_idx), w, slots, shared)``."""
-    _cuda(topk_idx, "topk_idx")
-    _req(topk_idx.dtype == torch.int64, "topk_idx must be int64")
-    _req(topk_idx.dim() == 2 and topk_idx.shape[1] > 0, "topk_idx must be [N, K]")
-    if not 0 < num_experts <= 1024:
-        raise RuntimeError(f"moe_group_rows supports 1 <= E <= 1024, got {num_experts}")
-    return _OPS.moe_group_rows(topk_idx.contiguous(), num_experts)
-
-
-def _linear_operands(x: torch.Tensor, weight: torch.Tensor):
-    _cuda(x, "x")
-    _dtype_code(x, "x")
-    _operand(weight, "weight", x)
-    _req(weight.dim() == 2, "weight must be [d_out, d_in]")
-    _req(x.dim() >= 1 and x.shape[-1] == weight.shape[1], "x must be [..., d_in]")
-    _req(weight.shape[0] > 0 and weight.shape[1] > 0, "weight must not be empty")
+    return _OPS.moe_group_rows(topk_idx, num_experts)
 
 
 def fused_linear_forward(x: torch.Tensor, weight: torch.Tensor, bias=None,
@@ -495,28 +458,7 @@ def fused_linear_forward(x: torch.Tensor, weight: torch.Tensor, bias=None,
     fp32. Sums, bias, activation and residual are fp32, rounded once. x and residual may be
     2-dimensional with any row stride. save_pre: also returns the values the activation took,
     [..., d_out], which fused_linear_backward needs for every activation but none."""
-    _linear_operands(x, weight)
-    d_out = weight.shape[0]
-    act = _act_code(activation, d_out)
-    bias = _bias(bias, x, (d_out,))
-    if residual is not None:
-        _operand(residual, "residual", x)
-        cols = d_out // 2 if activation == "swiglu" else d_out
-        _req(residual.shape[:-1] == x.shape[:-1] and residual.dim() == x.dim()
-             and residual.shape[-1] == cols, f"residual must be [..., {cols}]")
-    return _OPS.fused_linear_forward(x, weight, bias, residual, act, int(save_pre))
-
-
-def _saved(dy: torch.Tensor, x: torch.Tensor, pre, lead: tuple, d_out: int, activation: str):
-    cols = d_out // 2 if activation == "swiglu" else d_out
-    _operand(dy, "dy", x)
-    _req(tuple(dy.shape) == (*lead, cols), f"dy must be {[*lead, cols]}, got {list(dy.shape)}")
-    if activation == "none":
-        return None
-    _req(pre is not None, f"pre is needed for activation {activation}")
-    _operand(pre, "pre", x)
-    _req(tuple(pre.shape) == (*lead, d_out), f"pre must be {[*lead, d_out]}, got {list(pre.shape)}")
-    return pre.contiguous()
+    return _OPS.fused_linear_forward(x, weight, bias, residual, _act_code(activation), save_pre)
 
 
 def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre=None,
@@ -525,23 +467,7 @@ def fused_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     None. The residual's gradient is dy. pre: the forward's (unused with activation none).
     dweight has weight's order of dimensions in memory. act'(pre) dy is rounded to x's dtype,
     which the matrix cores take, before its products and sums."""
-    _linear_operands(x, weight)
-    act = _act_code(activation, weight.shape[0])
-    pre = _saved(dy, x, pre, tuple(x.shape[:-1]), weight.shape[0], activation)
-    return _OPS.fused_linear_backward(dy.contiguous(), x, weight, pre, act, int(bias))
-
-
-def _grouped_operands(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, rows):
-    _cuda(x, "x")
-    _dtype_code(x, "x")
-    _operand(weight, "weight", x)
-    _req(weight.dim() == 3, "weight must be [E, d_in, d_out]")
-    E, d_in, d_out = weight.shape
-    _req(x.dim() == 2 and x.shape[1] == d_in, "x must be [R, d_in]")
-    _req(E > 0 and d_in > 0 and d_out > 0, "weight must not be empty")
-    offsets = _index(offsets, "offsets", x)
-    _req(offsets.numel() == E + 1, "offsets must have E + 1 elements")
-    return offsets, None if rows is None else _index(rows, "rows", x)
+    return _OPS.fused_linear_backward(dy, x, weight, pre, _act_code(activation), bias)
 
 
 def grouped_linear_forward(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
@@ -554,11 +480,8 @@ def grouped_linear_forward(x: torch.Tensor, weight: torch.Tensor, offsets: torch
     [M, d_out] (swiglu: d_out / 2). Rows past offsets[E] are zeros, and so is a row of x that
     an index outside it names. Activations, bias and save_pre as fused_linear_forward's, bias
     [E, d_out]."""
-    offsets, rows = _grouped_operands(x, weight, offsets, rows)
-    E, _, d_out = weight.shape
-    act = _act_code(activation, d_out)
-    bias = _bias(bias, x, (E, d_out))
-    return _OPS.grouped_linear_forward(x, weight, offsets, rows, bias, act, int(save_pre))
+    return _OPS.grouped_linear_forward(x, weight, offsets, rows, bias, _act_code(activation),
+                                       save_pre)
 
 
 def grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
@@ -568,9 +491,5 @@ def grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Ten
     past offsets[E]): the gradient of a row of x that several rows name is their sum, with
     moe_group_rows' plan ``moe_dispatch_backward(dx[None], torch.zeros_like(topk_idx), slots,
     N, d_in)``. dweight is zero for groups without rows; dbias [E, d_out] when bias."""
-    offsets, rows = _grouped_operands(x, weight, offsets, rows)
-    M = x.shape[0] if rows is None else rows.numel()
-    act = _act_code(activation, weight.shape[2])
-    pre = _saved(dy, x, pre, (M,), weight.shape[2], activation)
-    return _OPS.grouped_linear_backward(dy.contiguous(), x, weight, offsets, rows, pre, act,
-                                        int(bias))
+    return _OPS.grouped_linear_backward(dy, x, weight, offsets, rows, pre, _act_code(activation),
+                                        bias)

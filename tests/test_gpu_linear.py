@@ -291,12 +291,64 @@ def test_linear_gradient_by_differences(pc, act):
             assert abs(num - float(g.reshape(-1)[k])) <= 2e-3 * float(g.abs().max())
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M,I,O", [(4096, 64, 2048), (4100, 136, 2056), (20000, 72, 264)])
+def test_linear_many_tiles(pc, M, I, O, dtype):
+    """Launches of the largest tiles: whole rounds of the chip, and last tiles that several
+    workgroups share (272 tiles: 2 an XCD; 632: ragged ends); residual, kept values, both
+    orders."""
+    dt = DT[dtype]
+    x, res = rand(M, I, seed=1, dt=dt), rand(M, O, seed=2, dt=dt)
+    dy = rand(M, O, seed=3, dt=dt)
+    w, b = rand(O, I, seed=4, dt=dt, scale=I ** -0.5), rand(O, seed=5, dt=dt)
+    for ww in (w, w.t().contiguous().t()):
+        for act in ("none", "gelu", "silu"):
+            y, pre = pc.fused_linear_forward(x, ww, b, act, residual=res, save_pre=True)
+            check_forward(y, pre, x, ww.t(), b, act, dt, res=res, what=act)
+        check_forward(pc.fused_linear_forward(x, ww), None, x, ww.t(), None, "none", dt)
+        dx, dw, db = pc.fused_linear_backward(dy, x, ww, pre, "silu", bias=True)
+        check_backward(dx, dw.t(), db, dy, x, ww.t(), pre, "silu", dt)
+
+
+@pytest.mark.parametrize("M,I,O", [(5, 64, 48), (300, 200, 264), (700, 1024, 520)])
+def test_linear_fp32_infinities(pc, M, I, O):
+    """fp32 sums with infinities, NaN and values beyond bf16's range are those of fp32: the same
+    finite results, infinities of the same sign and NaNs as torch's products."""
+    x, w = rand(M, I, seed=1, dt=torch.float32), rand(O, I, seed=2, dt=torch.float32)
+    x[1, 3], x[2, 5], x[3, 7], x[4, 1] = float("inf"), -float("inf"), float("nan"), 3.4e38
+    w[:, 1] *= 0.25
+    w[7, 9] = 3.4e38
+    x[0, 9] = 0.0
+    dy = rand(M, O, seed=3, dt=torch.float32)
+    y = pc.fused_linear_forward(x, w)
+    dx, dw, db = pc.fused_linear_backward(dy, x, w, bias=True)
+    ref = x.double() @ w.double().t()
+    for got, a, b in ((y, x.double(), w.double().t()), (dx, dy.double(), w.double()),
+                      (dw, dy.double().t(), x.double())):
+        want = a @ b
+        n = a.shape[1] + 2
+        # a finite product past fp32's range is an infinity in fp32 and not in 64 bits: with one of
+        # the other sign in the sum it gives NaN (inf - inf), without one an infinity. Sums that
+        # hold such a product have no 64-bit counterpart. Magnitudes: the sum of the finite
+        # factors' products bounds each of them.
+        fa, fb = (torch.where(t.isfinite(), t, 0.0) for t in (a, b))
+        S = fa.abs() @ fb.abs()
+        there = S < 3.4e38
+        fin = torch.isfinite(want) & there
+        assert bool(((got.double() - want)[fin].abs() <= n * U * S[fin] + U * want[fin].abs()).all())
+        assert torch.equal(got.isnan() & there, want.isnan() & there)
+        inf = torch.isinf(want) & there
+        assert torch.equal(got[inf].double(), want[inf])
+        assert bool(there.any())
+    assert ref.isnan().any() and torch.isinf(ref).any()
+
+
 # --------------------------------------------------------------------------------------
 # grouped_linear
 # --------------------------------------------------------------------------------------
 
 COUNTS = [[5], [0, 3, 0], [1] * 7, [64, 0, 65, 1, 130], [0, 0], [300, 17, 0, 128, 2, 63],
-          [3, 0] * 40 + [129], [1] * 130]
+          [3, 0] * 40 + [129], [1] * 130, [4000, 100, 0, 5200, 257]]
 
 
 @pytest.mark.parametrize("dtype", list(DT))

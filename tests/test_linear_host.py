@@ -10,27 +10,21 @@ import torch
 
 
 @pytest.fixture
-def pc(monkeypatch):
-    """pulsar_cuda with its device checks stubbed, so that CPU tensors stand in, and a native half
-    that must not be reached."""
+def pc():
     import pulsar_cuda
 
-    class NoLib:
-        def __getattr__(self, name):
-            raise AssertionError(f"library called: {name}")
-
-    monkeypatch.setattr(pulsar_cuda, "_OPS", NoLib())
-    monkeypatch.setattr(pulsar_cuda, "_cuda", lambda t, n: None)
     return pulsar_cuda
 
 
 def _refuses(pc, fn, base, cases):
+    """Types and shapes are refused with a message before the device is looked at, which refuses
+    the base call itself here: its tensors are on the CPU."""
     for msg, over in cases:
         args = dict(base, **over)
         with pytest.raises(RuntimeError, match=msg):
             getattr(pc, fn)(**args)
-    with pytest.raises(AssertionError, match="library called"):
-        getattr(pc, fn)(**base)  # the base call itself is taken
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        getattr(pc, fn)(**base)
 
 
 def test_group_rows_refusals(pc):
@@ -62,8 +56,8 @@ def test_fused_linear_refusals(pc):
     _refuses(pc, "fused_linear_forward", base, common + [
         ("bias must have the dtype", dict(bias=torch.zeros(6, dtype=torch.float64))),
         (r"bias must be \[6\]", dict(bias=torch.zeros(8, dtype=bf))),
-        (r"residual must be \[\.\.\., 6\]", dict(residual=torch.zeros(5, 8, dtype=bf))),
-        (r"residual must be \[\.\.\., 3\]", dict(residual=torch.zeros(5, 6, dtype=bf),
+        (r"residual must be \[5, 6\]", dict(residual=torch.zeros(5, 8, dtype=bf))),
+        (r"residual must be \[5, 3\]", dict(residual=torch.zeros(5, 6, dtype=bf),
                                                  activation="swiglu")),
         ("residual must have the dtype", dict(residual=torch.zeros(5, 6))),
     ])
@@ -72,7 +66,7 @@ def test_fused_linear_refusals(pc):
         (r"dy must be \[5, 6\]", dict(dy=dy[:4])),
         (r"dy must be \[5, 3\]", dict(activation="swiglu", pre=dy)),
         ("dy must have the dtype", dict(dy=dy.float())),
-        ("pre is needed for activation gelu", dict(activation="gelu")),
+        ("pre is needed for every activation but none", dict(activation="gelu")),
         (r"pre must be \[5, 6\]", dict(activation="gelu", pre=dy[:, :3])),
     ])
 
