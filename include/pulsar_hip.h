@@ -235,7 +235,9 @@ int pulsar_causal_conv1d_k4_backward(const void* dout, const void* x, const floa
  *   bf16 and fp32; fp32 sums; pre-activation values, bias, activation and residual are taken
  *   in fp32 and each output is rounded once. The gradients take act'(pre) dy rounded to the
  *   activation dtype into their products. Same inputs give the same bits on every call.
- *   1 <= d_in, d_out, 1 <= groups <= 65536, rows < 2^31 - 256.
+ *   1 <= d_in, d_out <= 2^30, 1 <= groups <= 65536, rows and row strides < 2^31 - 256. fp32
+ *   products run on the bf16 matrix cores in three exact parts (each within half a step of
+ *   fp32) and again in fp32 where a sum is not finite.
  * ------------------------------------------------------------------------------- */
 
 /* moe_group_rows(topk_idx, E): the assignments [N, K] sorted by expert, stable.

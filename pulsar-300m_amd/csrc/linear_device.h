@@ -533,6 +533,12 @@ __device__ __forceinline__ bool place_tile(int tiles_r, int tiles_c, int& tr, in
 // The same where the last tiles of an XCD's range, those past whole rounds of its CUs, may be shared:
 // `parts` workgroups a tile.
 constexpr int kXcdCus = 32;
+__host__ __device__ inline int shared_parts(int rest) { return rest * 4 <= kXcdCus ? 4 : rest * 2 <= kXcdCus ? 2 : 1; }
+// Workgroups for a range of `count` tiles.
+__host__ __device__ inline int shared_slots(int count) {
+  const int rest = count % kXcdCus;
+  return count - rest + rest * shared_parts(rest);
+}
 __device__ __forceinline__ bool place_shared(int tiles_r, int tiles_c, int& tr, int& tc, int& part,
                                              int& parts) {
   const int total = tiles_r * tiles_c, xcd = (int)blockIdx.x % kXcds, slot = (int)blockIdx.x / kXcds;
@@ -543,7 +549,7 @@ __device__ __forceinline__ bool place_shared(int tiles_r, int tiles_c, int& tr, 
   part = 0;
   parts = 1;
   if (slot >= whole) {
-    parts = rest * 4 <= kXcdCus ? 4 : rest * 2 <= kXcdCus ? 2 : 1;
+    parts = shared_parts(rest);
     item = whole + (slot - whole) / parts;
     part = (slot - whole) % parts;
   }
@@ -555,7 +561,9 @@ __device__ __forceinline__ bool place_shared(int tiles_r, int tiles_c, int& tr, 
 // Weight-gradient tiles: group by group, the largest groups first (up to 64 groups), so that the
 // long sums start early and the short ones fill up behind them; a group's tiles go to the XCDs
 // in runs of an eighth of them, so that every XCD gets its share of every group.
-__device__ __forceinline__ int wgrad_run(int tiles_of_group) { return max(1, tiles_of_group / kXcds); }
+__host__ __device__ inline int wgrad_run(int tiles_of_group) {
+  return tiles_of_group < kXcds ? 1 : tiles_of_group / kXcds;
+}
 __device__ __forceinline__ bool place_wgrad(const LinearArgs& a, int& group, int& split, int& mt, int& nt) {
   const int per_split = a.tiles_m * a.tiles_n, per = per_split * a.splits, c = wgrad_run(per);
   const int xcd = (int)blockIdx.x % kXcds, slot = (int)blockIdx.x / kXcds;

@@ -292,11 +292,11 @@ def test_linear_gradient_by_differences(pc, act):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("M,I,O", [(4096, 64, 2048), (4100, 136, 2056), (20000, 72, 264)])
+@pytest.mark.parametrize("M,I,O", [(4096, 64, 2048), (20000, 72, 264), (16384, 1024, 1024),
+                                   (36001, 1024, 1000), (38500, 1024, 1024)])
 def test_linear_many_tiles(pc, M, I, O, dtype):
-    """Launches of the largest tiles: whole rounds of the chip, and last tiles that several
-    workgroups share (272 tiles: 2 an XCD; 632: ragged ends); residual, kept values, both
-    orders."""
+    """Launches of many tiles of every shape: whole rounds of the chip, and last tiles that two or
+    four workgroups share (1024 wide); residual, kept values, both orders."""
     dt = DT[dtype]
     x, res = rand(M, I, seed=1, dt=dt), rand(M, O, seed=2, dt=dt)
     dy = rand(M, O, seed=3, dt=dt)
@@ -306,6 +306,7 @@ def test_linear_many_tiles(pc, M, I, O, dtype):
             y, pre = pc.fused_linear_forward(x, ww, b, act, residual=res, save_pre=True)
             check_forward(y, pre, x, ww.t(), b, act, dt, res=res, what=act)
         check_forward(pc.fused_linear_forward(x, ww), None, x, ww.t(), None, "none", dt)
+        check_forward(pc.fused_linear_forward(x, ww, b, "swiglu"), None, x, ww.t(), b, "swiglu", dt)
         dx, dw, db = pc.fused_linear_backward(dy, x, ww, pre, "silu", bias=True)
         check_backward(dx, dw.t(), db, dy, x, ww.t(), pre, "silu", dt)
 
@@ -348,7 +349,7 @@ def test_linear_fp32_infinities(pc, M, I, O):
 # --------------------------------------------------------------------------------------
 
 COUNTS = [[5], [0, 3, 0], [1] * 7, [64, 0, 65, 1, 130], [0, 0], [300, 17, 0, 128, 2, 63],
-          [3, 0] * 40 + [129], [1] * 130, [4000, 100, 0, 5200, 257]]
+          [3, 0] * 40 + [129], [1] * 130, [2] * 63, [3] * 64, [4000, 100, 0, 5200, 257]]
 
 
 @pytest.mark.parametrize("dtype", list(DT))
@@ -403,6 +404,34 @@ def test_grouped(pc, counts, I, O, order, gather, dtype):
         for p, r in zip((dx, dw, db), pc.grouped_linear_backward(dy, x, w, offsets, rows, pre, act,
                                                                  bias=True)):
             assert torch.equal(p, r)
+
+
+@pytest.mark.parametrize("order", ["io", "oi"])
+def test_grouped_many_rows(pc, order):
+    """50,000 rows in uneven groups: the largest tiles, the last of them shared, group ends inside
+    shared tiles, gathered rows."""
+    dt, I, O = torch.bfloat16, 1024, 1024
+    counts = [20011, 0, 7, 9000, 256, 12345, 1, 8421]
+    M, R = sum(counts), 9000
+    offsets = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32).cuda()
+    rows = torch.randint(0, R, (M + 40,), generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    x, w = rand(R, I, seed=2, dt=dt), rand(len(counts), I, O, seed=3, dt=dt, scale=I ** -0.5)
+    if order == "oi":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    for act in ("none", "swiglu"):
+        y, pre = pc.grouped_linear_forward(x, w, offsets, rows, None, act, save_pre=True)
+        dy = rand(*y.shape, seed=4, dt=dt)
+        dx, dw, db = pc.grouped_linear_backward(dy, x, w, offsets, rows, pre, act, bias=True)
+        assert not y[M:].any() and not pre[M:].any() and not dx[M:].any()
+        s = 0
+        for e, c in enumerate(counts):
+            q, s = slice(s, s + c), s + c
+            if c == 0:
+                assert not dw[e].any()
+                continue
+            xs = x[rows[q].long()]
+            check_forward(y[q], pre[q], xs, w[e], None, act, dt, what=f"group {e}")
+            check_backward(dx[q], dw[e], db[e], dy[q], xs, w[e], pre[q], act, dt, what=f"group {e}")
 
 
 @pytest.mark.parametrize("dtype", list(DT))
