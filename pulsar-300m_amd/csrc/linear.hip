@@ -570,6 +570,11 @@ struct Call {
       return fail(PULSAR_ERR_INVALID, std::string(what) + ": rows of x overlap");
     return PULSAR_OK;
   }
+  // The workspace's size does not depend on the index, so only the calls look at it.
+  int check_rows() const {
+    return index || x_rows == rows ? PULSAR_OK
+                                   : fail(PULSAR_ERR_INVALID, std::string(what) + ": without an index x must have `rows` rows");
+  }
   int null_pointer() const { return fail(PULSAR_ERR_INVALID, std::string(what) + ": null pointer"); }
   int no_workspace() const {
     return fail(PULSAR_ERR_INVALID, std::string(what) + ": workspace missing or not 16-byte aligned");
@@ -588,7 +593,8 @@ struct ForwardPlan {
 
 int forward(const Call& c, const void* bias, int bias_dtype, const void* residual, int64_t res_rs,
             void* y, void* pre, void* workspace, hipStream_t s) {
-  const int rc = c.check();
+  int rc = c.check();
+  if (rc == PULSAR_OK) rc = c.check_rows();
   if (rc != PULSAR_OK) return rc;
   if (bias && bias_dtype != PULSAR_F32 && bias_dtype != PULSAR_BF16)
     return fail(PULSAR_ERR_INVALID, std::string(c.what) + ": bias dtype must be PULSAR_F32 or PULSAR_BF16");
@@ -687,7 +693,8 @@ int backward_t(const Call& c, const BackwardPlan& plan, const void* dy, const vo
 
 int backward(const Call& c, const void* dy, const void* pre, void* dx, void* dw, void* db,
              void* workspace, hipStream_t s) {
-  const int rc = c.check();
+  int rc = c.check();
+  if (rc == PULSAR_OK) rc = c.check_rows();
   if (rc != PULSAR_OK) return rc;
   if (!dw || (c.rows > 0 && (!dy || (!c.x && c.x_rows > 0) || !c.w.p || !dx ||
                              (c.act != PULSAR_ACT_NONE && !pre))))

@@ -177,3 +177,19 @@ def test_c_entries_refuse_before_any_launch():
                                               2, 8, 6, 0, bf, None, None), b"workspace")
     refused(lib.pulsar_grouped_linear_backward(p, p, 8, 4, None, None, p, 48, 6, 1, None, p, p, None,
                                                4, 2, 8, 6, 0, bf, None, None), b"null")
+
+
+def test_rows_of_x_without_an_index():
+    """Row i is then x's row i: fewer rows of x than rows of y would be read past their end."""
+    from pulsar_cuda import _lib
+
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 15) // 16 * 16)
+    for x_rows in (0, 3, 5):
+        assert lib.pulsar_grouped_linear_forward(p, 8, x_rows, None, p, p, 64, 8, 1, None, 0, p, None, 4, 2,
+                                                 8, 8, 0, _lib.PULSAR_BF16, None, None) != 0
+        assert b"without an index" in lib.pulsar_last_error()
+        assert lib.pulsar_grouped_linear_backward(p, p, 8, x_rows, None, p, p, 64, 8, 1, None, p, p, None,
+                                                  4, 2, 8, 8, 0, _lib.PULSAR_BF16, None, None) != 0
+        assert b"without an index" in lib.pulsar_last_error()
