@@ -267,9 +267,9 @@ __global__ void __launch_bounds__(256) linear_act_grad_kernel(const T* pre, cons
       float u[W], ou[W];
       load_run<W>(pre + r * N + f + c, u, n);
 #pragma unroll
-      for (int q = 0; q < W; ++q) {
-        ou[q] = d[q] * g[q] * fast_sigmoid(g[q]);
-        o[q] = d[q] * u[q] * act_slope(PULSAR_ACT_SILU, g[q]);
+      for (int q = 0; q < W; ++q) {  // dy last: dy g may pass fp32's range where dy silu(g) does not
+        ou[q] = d[q] * (g[q] * fast_sigmoid(g[q]));
+        o[q] = d[q] * (u[q] * act_slope(PULSAR_ACT_SILU, g[q]));
       }
       store_run<W>(out + f + c, ou, n);
     } else {

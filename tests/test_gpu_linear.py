@@ -231,6 +231,25 @@ def test_activation_gradient_at_the_ends(pc, act):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+def test_swiglu_gradient_of_large_dy(pc, dtype):
+    """dy g and dy u pass fp32's range where the gradients, dy silu(g) and dy u silu'(g), are far
+    inside it. One row: the bias gradient is dpre itself."""
+    dt = DT[dtype]
+    g = torch.tensor([-200.0, -60.0, -60.0, -200.0])
+    u = torch.tensor([1000.0, 1000.0, -1000.0, 0.0])
+    pre = torch.cat([g, u])[None].to(dt).cuda()
+    dy = torch.tensor([[1e37, 1e37, -1e37, 3e38]]).to(dt).cuda()
+    x, w = rand(1, 8, seed=1, dt=dt), torch.zeros(8, 8, dtype=dt, device="cuda")
+    dx, dw, db = pc.fused_linear_backward(dy, x, w, pre, "swiglu", True)
+    want, e = dpre64("swiglu", pre, dy)
+    # e^g's argument is rounded to |g| u relative, more than e's share of dy u for |g| = 60; and
+    # what fp32's exponent range cannot hold (e^-200 is 0) is below 2^-126 of the other factors
+    e = 1e-4 * want.abs() + 2.0 ** -100 * (dy.double().abs().repeat(1, 2))
+    check(db[None], want, half(dt) * (want.abs() + e) + e, "db")
+    assert not dx.any() and torch.isfinite(dw).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_linear_strided_operands(pc, dtype):
     """x, residual and weight as column slices of wider buffers, aligned and not; what lies
     beside them (NaN) is not read into any result."""
@@ -582,3 +601,20 @@ def test_offsets_past_32_bits(pc):
     assert y.numel() > 2 ** 31
     check_forward(y[-64:], None, x[-64:], w.t(), None, "none", dt)
     assert torch.equal(y[-64:], y[:64]) and torch.equal(y[2 ** 20:2 ** 20 + 64], y[:64])
+
+
+@pytest.mark.parametrize("I", [64, 777, 4096])
+@pytest.mark.parametrize("M", [3, 200])
+def test_linear_fp32_small_values(pc, M, I):
+    """Products far below one, from operands of 2^-55 each and of 2^-100 by 1, keep fp32's precision:
+    the parts an operand is cut into, and their products, are not lost below bf16's range or
+    fp32's normal numbers. Scaling by powers of two changes no bound but for subnormal
+    products, each of the six per term within 2^-149, and for subnormal last parts, 2^-134."""
+    for a, b in ((-55, -55), (-100, 0), (0, -100)):
+        x = rand(M, I, seed=M + I, dt=torch.float32) * 2.0 ** a
+        w = rand(264, I, seed=I, dt=torch.float32) * 2.0 ** b
+        y = pc.fused_linear_forward(x, w)
+        want = x.double() @ w.double().t()
+        t = (I + 2) * U * (x.double().abs() @ w.double().abs().t()) + 6 * I * 2.0 ** -149
+        t += 2.0 ** -134 * (x.double().abs().sum(1, keepdim=True) + w.double().abs().sum(1))
+        check(y, want, U * (want.abs() + t) + t, f"2^{a} 2^{b}")
