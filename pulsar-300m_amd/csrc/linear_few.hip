@@ -46,6 +46,9 @@ __device__ __forceinline__ void slab_write_tile(float* slab, const lin_f32x4 (&a
 // end. Weights that are contiguous along k go from memory straight into matrix-core order; bf16
 // weights contiguous along the output columns pass through the wave's own corner of LDS and its
 // transposing read; fp32 ones are loaded a column run per lane, tiles sharing a run.
+//   Bound by the latency of a few dependent loads (offsets, row index, operands), and from some
+// hundred rows by what a CU streams: 16 rows x 1024 x 1024 in bf16 5.9 us with 64 workgroups (2.2
+// MB), 4 experts of one row 6.6 us (8.4 MB, 1.3 TB/s), 517 x 777 by 1023 k 12 us.
 template <typename T, bool BKC, bool PAIR, int RT, int CT, int W, int D>
 __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
   typedef typename Frag<T>::type F;
