@@ -237,7 +237,7 @@ int pulsar_causal_conv1d_k4_backward(const void* dout, const void* x, const floa
  *   activation dtype into their products. Same inputs give the same bits on every call.
  *   1 <= d_in, d_out <= 2^30, 1 <= groups <= 65536, rows and row strides < 2^31 - 256. fp32
  *   products run on the bf16 matrix cores in three exact parts (each within half a step of
- *   fp32) and again in fp32 where a sum is not finite.
+ *   fp32; operands below 2^-110 within 2^-134) and again in fp32 where a sum is not finite.
  * ------------------------------------------------------------------------------- */
 
 /* moe_group_rows(topk_idx, E): the assignments [N, K] sorted by expert, stable.
@@ -257,7 +257,8 @@ int pulsar_moe_group_rows(const int64_t* topk_idx, int32_t* offsets, int32_t* ro
  *   [rows, d_out], the values the activation took, for the backward call, nullable.
  *   workspace: the given number of bytes (-1: bad arguments) of device memory, 16-byte aligned,
  *   any contents; none when it is 0. Operands whose rows are not made of whole, aligned 16-byte
- *   chunks are copied into it first (the pointers are only looked at). */
+ *   chunks are copied into it first (the pointers are only looked at), and dense products with
+ *   few tiles and a long k keep partial sums there. */
 int64_t pulsar_fused_linear_forward_workspace_bytes(const void* x, int64_t x_rs, const void* w,
                                                     int64_t w_out, int64_t w_in, int64_t rows,
                                                     int64_t d_in, int64_t d_out, int activation,

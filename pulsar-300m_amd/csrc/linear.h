@@ -37,9 +37,9 @@ struct LinearArgs {
   int64_t ldr;
   int act;
   void* db;                // weight gradient: [groups][dim] sums of dpre's rows, storage type
-  float* part;             // weight gradient in splits: [split][groups][M][N] partial sums
-  float* part_db;          //   and [split][groups][dim]
-  int splits;
+  int splits;              // workgroups that share a sum over k; with several, partial sums:
+  float* part;             //   weight gradient: [split][groups][M][N], products (dense): [split][rows][N]
+  float* part_db;          //   weight gradient: [split][groups][dim]
   int tiles_m, tiles_n;    // weight gradient: tiles of one group
   int max_tiles;           // products: bound of the row tiles
 };
@@ -50,6 +50,14 @@ struct FewShape {
   int rt, ct;
 };
 constexpr FewShape kFewShapes[6] = {{1, 1}, {1, 2}, {2, 2}, {1, 4}, {2, 4}, {4, 4}};
+// Few or many, a split of k is whole chunks of 128 bytes: the k's [first, first + count) of split `s`.
+template <typename T>
+__host__ __device__ inline void split_range(int K, int splits, int s, int& first, int& count) {
+  constexpr int BK = 128 / (int)sizeof(T);
+  const int per = ((K + splits - 1) / splits + BK - 1) / BK * BK;
+  first = (int)((int64_t)s * per < K ? (int64_t)s * per : K);
+  count = K - first < per ? K - first : per;
+}
 int launch_linear_few(LinearArgs& a, int dtype, bool b_kc, int shape, hipStream_t s);
 
 // Sigmoid by the exponential and reciprocal instructions: each within one step of fp32, the

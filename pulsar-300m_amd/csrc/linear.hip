@@ -29,10 +29,12 @@ __device__ __forceinline__ void rows_tile(const LinearArgs& a, uint4* lds, int t
   constexpr int OBN = PAIR ? BN / 2 : BN;      // output columns of a tile
   const int n0 = tc * OBN;
   const bool none = group >= a.groups;  // rows of no group: zeros
-  const int K = none ? 0 : a.K;
+  constexpr bool SPLIT = !SH::kShared;
+  int kfirst = 0, K = none ? 0 : a.K;
+  if (SPLIT && a.part) split_range<T>(K, a.splits, (int)blockIdx.y, kfirst, K);
 
-  const T* A = reinterpret_cast<const T*>(a.A);
-  const T* B = reinterpret_cast<const T*>(a.B) + (none ? 0 : group) * a.b_group;
+  const T* A = reinterpret_cast<const T*>(a.A) + kfirst;
+  const T* B = reinterpret_cast<const T*>(a.B) + (none ? 0 : group) * a.b_group + kfirst * (BKC ? 1 : a.ldb);
   OA oa;
   oa.init_kc([&](int r) -> const T* {
     int64_t i = min(r0 + r, r1 - 1);
@@ -91,7 +93,7 @@ __device__ __forceinline__ void rows_tile(const LinearArgs& a, uint4* lds, int t
   __syncthreads();  // the tiles' memory now holds the epilogue's rows
   const Slab slab{reinterpret_cast<float*>(lds) + wv * Slab::kFloats};
   const EpilogueBias<T, MAP, PAIR> bias(a, group, none, n0 + col_w, f);
-  rows_epilogue<T, MAP, BW, PAIR>(a, acc, slab, bias, none, r0 + row_w, r1, n0 + col_w, f);
+  rows_epilogue<T, MAP, BW, PAIR, SPLIT>(a, acc, slab, bias, none, r0 + row_w, r1, n0 + col_w, f);
 }
 
 // One workgroup a tile. With one workgroup a CU (256 x 256) the tiles that do not fill a whole
@@ -236,6 +238,32 @@ __global__ void __launch_bounds__(SH::kThreads, SH::WPS) linear_wgrad_kernel(Lin
   wgrad_epilogue<T, MAP, BWR, BWC, SIDE>(a, acc, sum[0], slab, sums, group, split, m0 + row_w, n0 + col_w);
 }
 
+// The epilogue of a dense product in splits: sums of the partial ones, in order. 8 columns a thread.
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(256) linear_finish_kernel(LinearArgs a) {
+  const int f = PAIR ? a.N / 2 : a.N, per = (f + 7) / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / per;
+  if (r >= a.rows) return;
+  const int col = (int)(i - r * per) * 8;
+  float bias[2][8], v[8], u[8];
+  load_bias<PAIR>(a, 0, false, col, f, bias);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = u[q] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.part + ((int64_t)s * a.rows + r) * a.N + col;
+    float x[8];
+    load_run<8>(p, x, f - col);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] += x[q];
+    if constexpr (PAIR) {
+      load_run<8>(p + f, x, f - col);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) u[q] += x[q];
+    }
+  }
+  finish_run<T, PAIR, false>(a, a.act, r, col, f, v, u, bias);
+}
+
 // Sums of a weight gradient's splits, in order; `count` elements of one split's partials, the
 // first `n_c` of them C's (contiguous), the rest db's. 8 splits of 1024 x 2048: 11 us, 71 MB in all.
 template <typename T>
@@ -353,7 +381,8 @@ int launch_rows_shape(LinearArgs& a, hipStream_t s) {
     else
       slots = std::max(shared_slots((int)slots), shared_slots((int)((tiles - 1) % slots + 1)));
   }
-  linear_rows_kernel<T, BKC, PAIR, SH><<<(unsigned)(slots * kXcds), SH::kThreads, 0, s>>>(a);
+  linear_rows_kernel<T, BKC, PAIR, SH>
+      <<<dim3((unsigned)(slots * kXcds), a.part ? a.splits : 1), SH::kThreads, 0, s>>>(a);
   PULSAR_LAUNCH_CHECK();
   return PULSAR_OK;
 }
@@ -369,48 +398,85 @@ int launch_rows_shape(LinearArgs& a, hipStream_t s) {
 // rows in 32 x 32 19.7 (18.6), 32 x 64 26 (25.9); 2048 rows in 64 x 128 12.6 (12.5); 16384 x 2048
 // x 1024 in 128 x 128 85 (87), in 256 x 256 77 (79). A ragged launch has about 0.6 partial tiles a
 // group, at least one, and no whole rounds: a quarter of one is added beyond the first.
-double rows_cost(const LinearArgs& a, bool half, int BM, int BN, double rate, double flop_rate,
-                 double each) {
-  double rt = (a.rows + BM - 1) / BM;
-  if (a.offsets)
-    rt = std::max<double>(std::min(a.groups, a.rows), (double)a.rows / BM + 0.6 * a.groups);
-  const double n = rt * ((a.N + BN - 1) / BN) / 256;
-  double rounds = a.offsets ? (n <= 1 ? 1 : n + 0.25) : std::ceil(n);
+// `splits` workgroups share a tile's sum, and their partial ones meet in a second launch.
+struct Sizes {
+  double rows, groups, N, K;
+  bool ragged, half, pair, b_kc;
+};
+double rows_cost(const Sizes& z, int BM, int BN, double rate, double flop_rate, double each, int splits) {
+  double rt = std::ceil(z.rows / BM);
+  if (z.ragged) rt = std::max(std::min(z.groups, z.rows), z.rows / BM + 0.6 * z.groups);
+  const double n = rt * std::ceil(z.N / BN) / 256;
+  double rounds = z.ragged ? (n <= 1 ? 1 : n + 0.25) : std::ceil(n * splits) / splits;
   if (each > 0) {  // shared tiles: a quarter of a round takes 0.45 of its time, a half 0.65
     const double rest = n - std::floor(n);
     rounds = std::floor(n) + (rest == 0 ? 0 : rest <= 0.25 ? 0.45 : rest <= 0.5 ? 0.65 : 1);
   }
-  const double bytes = (double)(BM + BN) * a.K * (half ? 2 : 4), flops = 2.0 * BM * BN * a.K;
-  return 4 + rounds * (each + std::max(bytes / rate, flops / flop_rate));
+  const double bytes = (BM + BN) * z.K * (z.half ? 2 : 4), flops = 2.0 * BM * BN * z.K;
+  const double merge = splits > 1 ? 5 + z.rows * z.N * 8 * splits / 4e6 : 0;
+  return 4 + rounds * (each + std::max(bytes / rate, flops / flop_rate)) + merge;
+}
+
+// How a product is cut: the shape that the model expects to be fastest, the few-row ones (0 - 5) or
+// the tiles (64 x 128, 128 x 128, 256 x 256), and the workgroups that share a sum over k, which takes
+// a second launch and their partial sums' way through memory (5 us and 4 MB/us). A split has to
+// save a sixth of the expected time in bf16 and 4 % in fp32, about what the model is off by there.
+// Unsplit and split, us: 256 rows x 4096 x 4096 in bf16 36 and 28, in fp32 100 and 65; 2331 x 1024 by
+// 4096 k in fp32 184 and 134, 64 x 1024 18.8 and 16.8; not split in bf16: 1 x 1024 by 4096 k 8.5 and
+// 11.4, 512 x 512 by 4096 13.8 and 18.2. Only dense products are split: ragged ones have the groups'
+// times as many tiles.
+struct RowsPlan {
+  int shape, splits;
+  int64_t part_bytes;
+};
+RowsPlan rows_plan(const Sizes& z) {
+  RowsPlan best = {-1, 1, 0};
+  double least = 0;
+  auto offer = [&](int id, int splits, double us) {
+    if (best.shape < 0 || us < least) best.shape = id, best.splits = splits, least = us;
+  };
+  const double gain = z.half ? 0.85 : 0.96;
+  for (int s = 1; s == 1 || (!z.ragged && s <= 16 && z.K >= 256 * s); ++s) {
+    if (s == 2 && (least *= gain) <= 9) break;  // the second launch alone leaves no gain
+    for (int i = z.pair ? 1 : 0; i < 6; ++i)
+      offer(i, s, rows_cost(z, 16 * kFewShapes[i].rt, 16 * kFewShapes[i].ct, 35e3,
+                            z.half ? 5e6 : z.b_kc ? 0.33e6 : 0.25e6, 0, s));
+    offer(6, s, rows_cost(z, 64, 128, 45e3, z.half ? 5e6 : 0.5e6, 0, s));
+    offer(7, s, rows_cost(z, 128, 128, 49e3, z.half ? 5e6 : 0.6e6, 0, s));
+    if (z.half && s == 1) offer(8, s, rows_cost(z, 256, 256, 38e3, 5e6, 10, s));
+  }
+  if (best.splits > 1) best.part_bytes = (int64_t)(best.splits * z.rows * z.N * 4);
+  return best;
 }
 
 template <typename T>
-int launch_rows(LinearArgs& a, bool b_kc, hipStream_t s) {
+int launch_rows(LinearArgs& a, const RowsPlan& plan, bool b_kc, hipStream_t s) {
   constexpr bool half = sizeof(T) == 2;
   const bool pair = a.act == PULSAR_ACT_SWIGLU;
-  // the shape that the model expects to be fastest: the few-row ones, then the tiles
-  int best = -1;
-  double least = 0;
-  auto offer = [&](int id, double us) {
-    if (best < 0 || us < least) best = id, least = us;
-  };
-  for (int i = pair ? 1 : 0; i < 6; ++i)
-    offer(i, rows_cost(a, half, 16 * kFewShapes[i].rt, 16 * kFewShapes[i].ct, 35e3,
-                       half ? 5e6 : b_kc ? 0.33e6 : 0.25e6, 0));
-  offer(6, rows_cost(a, half, 64, 128, 45e3, half ? 5e6 : 0.5e6, 0));
-  offer(7, rows_cost(a, half, 128, 128, 49e3, half ? 5e6 : 0.6e6, 0));
-  if (half) offer(8, rows_cost(a, half, 256, 256, 38e3, 5e6, 10));
-  if (best < 6) return launch_linear_few(a, half ? PULSAR_BF16 : PULSAR_F32, b_kc, best, s);
+  a.splits = plan.splits;
   auto go = [&](auto kc, auto pr) {
     constexpr bool KC = decltype(kc)::value, P = decltype(pr)::value;
     if constexpr (half) {
-      if (best == 8) return launch_rows_shape<T, KC, P, LinWide>(a, s);
+      if (plan.shape == 8) return launch_rows_shape<T, KC, P, LinWide>(a, s);
     }
-    return best == 7 ? launch_rows_shape<T, KC, P, LinLarge>(a, s)
-                     : launch_rows_shape<T, KC, P, LinSmall>(a, s);
+    return plan.shape == 7 ? launch_rows_shape<T, KC, P, LinLarge>(a, s)
+                           : launch_rows_shape<T, KC, P, LinSmall>(a, s);
   };
-  if (b_kc) return pair ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
-  return pair ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
+  int rc;
+  if (plan.shape < 6)
+    rc = launch_linear_few(a, half ? PULSAR_BF16 : PULSAR_F32, b_kc, plan.shape, s);
+  else if (b_kc)
+    rc = pair ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  else
+    rc = pair ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
+  if (rc != PULSAR_OK || !a.part) return rc;
+  const int64_t n = (int64_t)a.rows * (((pair ? a.N / 2 : a.N) + 7) / 8);
+  if (pair)
+    linear_finish_kernel<T, true><<<blocks_for(n, 256), 256, 0, s>>>(a);
+  else
+    linear_finish_kernel<T, false><<<blocks_for(n, 256), 256, 0, s>>>(a);
+  PULSAR_LAUNCH_CHECK();
+  return PULSAR_OK;
 }
 
 // How a weight gradient is cut: tile shape and splits of the sum over rows. Splits: enough
@@ -560,11 +626,16 @@ struct Call {
   int64_t x_rs, x_rows;
   const int32_t* index;
   const int32_t* offsets;
+  bool ragged;
   Weight w;
   int64_t rows, groups, d_in, d_out;
   int act, dtype;
   const char* what;
 
+  Sizes sizes(int64_t N, int64_t K, bool pair, bool b_kc) const {
+    return {(double)rows, (double)groups, (double)N, (double)K, ragged, dtype == PULSAR_BF16,
+            pair, b_kc};
+  }
   int es() const { return dtype == PULSAR_BF16 ? 2 : 4; }
   Matrix x_matrix() const { return {x, x_rs, 0, 1, x_rows, d_in}; }
   Matrix w_matrix(bool pair) const {
@@ -597,9 +668,13 @@ struct ForwardPlan {
   Space ws;
   Packing pack;
   Matrix x, w;
+  RowsPlan rows;
+  float* part;
   ForwardPlan(const Call& c, void* workspace)
       : ws{static_cast<char*>(workspace)}, pack(c.es(), ws), x(pack(c.x_matrix())),
-        w(pack(c.w_matrix(c.act == PULSAR_ACT_SWIGLU))) {}
+        w(pack(c.w_matrix(c.act == PULSAR_ACT_SWIGLU))),
+        rows(rows_plan(c.sizes(c.d_out, c.d_in, c.act == PULSAR_ACT_SWIGLU, in_contiguous(c.w)))),
+        part(rows.part_bytes ? static_cast<float*>(ws.take(rows.part_bytes)) : nullptr) {}
 };
 
 int forward(const Call& c, const void* bias, int bias_dtype, const void* residual, int64_t res_rs,
@@ -628,18 +703,21 @@ int forward(const Call& c, const void* bias, int bias_dtype, const void* residua
   a.bias = bias; a.bias_dtype = bias_dtype;
   a.residual = residual; a.ldr = res_rs;
   a.act = c.act;
-  return c.dtype == PULSAR_BF16 ? launch_rows<bf16>(a, kc, s) : launch_rows<float>(a, kc, s);
+  a.part = plan.part;
+  return c.dtype == PULSAR_BF16 ? launch_rows<bf16>(a, plan.rows, kc, s) : launch_rows<float>(a, plan.rows, kc, s);
 }
 
 struct BackwardPlan {
   Space ws;
   Packing pack;
   Matrix x, w, dpre;
+  RowsPlan rows;
   WgradPlan wgrad;
-  float *part = nullptr, *part_db = nullptr;
+  float *part = nullptr, *part_db = nullptr;  // of the weight gradient; dx's lie there first
   BackwardPlan(const Call& c, const void* dy, void* workspace)
       : ws{static_cast<char*>(workspace)}, pack(c.es(), ws), x(pack(c.x_matrix())),
         w(pack(c.w_matrix(false))), dpre{dy, c.d_out, 0, 1, c.rows, c.d_out},
+        rows(rows_plan(c.sizes(c.d_in, c.d_out, false, !in_contiguous(c.w)))),
         wgrad(wgrad_plan(c.rows, c.groups, c.d_in, c.d_out, c.dtype)) {
     if (c.act == PULSAR_ACT_NONE) {
       dpre = pack(dpre);
@@ -647,10 +725,9 @@ struct BackwardPlan {
       dpre.ld = round_up(c.d_out, 16 / c.es());
       dpre.p = ws.take(c.rows * dpre.ld * c.es());
     }
-    if (wgrad.splits > 1) {
-      part = static_cast<float*>(ws.take(wgrad.splits * c.groups * c.d_in * c.d_out * 4));
-      part_db = static_cast<float*>(ws.take(wgrad.splits * c.groups * c.d_out * 4));
-    }
+    const int64_t n = wgrad.splits > 1 ? wgrad.splits * c.groups * c.d_in * c.d_out * 4 : 0;
+    if (n || rows.part_bytes) part = static_cast<float*>(ws.take(std::max(n, rows.part_bytes)));
+    if (n) part_db = static_cast<float*>(ws.take(wgrad.splits * c.groups * c.d_out * 4));
   }
 };
 
@@ -677,7 +754,8 @@ int backward_t(const Call& c, const BackwardPlan& plan, const void* dy, const vo
     a.offsets = c.offsets; a.groups = (int)c.groups; a.rows = (int)c.rows;
     a.N = (int)c.d_in; a.K = (int)c.d_out;
     a.C = dx; a.ldc = c.d_in;
-    const int rc = launch_rows<T>(a, !kc, s);
+    if (plan.rows.splits > 1) a.part = plan.part;
+    const int rc = launch_rows<T>(a, plan.rows, !kc, s);
     if (rc != PULSAR_OK) return rc;
   }
   // dw in the weight's own order: its contiguous dimension is n
@@ -735,7 +813,7 @@ int64_t pulsar_fused_linear_forward_workspace_bytes(const void* x, int64_t x_rs,
                                                     int64_t w_out, int64_t w_in, int64_t rows,
                                                     int64_t d_in, int64_t d_out, int activation,
                                                     int dtype) {
-  return forward_bytes(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
+  return forward_bytes(Call{x, x_rs, rows, nullptr, nullptr, false, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
                             d_out, activation, dtype, "fused_linear_forward"});
 }
 
@@ -744,7 +822,7 @@ int pulsar_fused_linear_forward(const void* x, int64_t x_rs, const void* w, int6
                                 const void* residual, int64_t residual_rs, void* y, void* pre,
                                 int64_t rows, int64_t d_in, int64_t d_out, int activation,
                                 int dtype, void* workspace, hipStream_t stream) {
-  return forward(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in, d_out,
+  return forward(Call{x, x_rs, rows, nullptr, nullptr, false, Weight{w, 0, w_in, w_out}, rows, 1, d_in, d_out,
                       activation, dtype, "fused_linear_forward"},
                  bias, bias_dtype, residual, residual_rs, y, pre, workspace, stream);
 }
@@ -753,7 +831,7 @@ int64_t pulsar_fused_linear_backward_workspace_bytes(const void* dy, const void*
                                                      const void* w, int64_t w_out, int64_t w_in,
                                                      int64_t rows, int64_t d_in, int64_t d_out,
                                                      int activation, int dtype) {
-  return backward_bytes(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
+  return backward_bytes(Call{x, x_rs, rows, nullptr, nullptr, false, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
                              d_out, activation, dtype, "fused_linear_backward"}, dy);
 }
 
@@ -761,7 +839,7 @@ int pulsar_fused_linear_backward(const void* dy, const void* x, int64_t x_rs, co
                                  int64_t w_out, int64_t w_in, const void* pre, void* dx, void* dw,
                                  void* db, int64_t rows, int64_t d_in, int64_t d_out,
                                  int activation, int dtype, void* workspace, hipStream_t stream) {
-  return backward(Call{x, x_rs, rows, nullptr, nullptr, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
+  return backward(Call{x, x_rs, rows, nullptr, nullptr, false, Weight{w, 0, w_in, w_out}, rows, 1, d_in,
                        d_out, activation, dtype, "fused_linear_backward"},
                   dy, pre, dx, dw, db, workspace, stream);
 }
@@ -771,7 +849,7 @@ int64_t pulsar_grouped_linear_forward_workspace_bytes(const void* x, int64_t x_r
                                                       int64_t w_out, int64_t rows, int64_t groups,
                                                       int64_t d_in, int64_t d_out, int activation,
                                                       int dtype) {
-  return forward_bytes(Call{x, x_rs, x_rows, nullptr, nullptr, Weight{w, w_group, w_in, w_out}, rows,
+  return forward_bytes(Call{x, x_rs, x_rows, nullptr, nullptr, true, Weight{w, w_group, w_in, w_out}, rows,
                             groups, d_in, d_out, activation, dtype, "grouped_linear_forward"});
 }
 
@@ -782,7 +860,7 @@ int pulsar_grouped_linear_forward(const void* x, int64_t x_rs, int64_t x_rows,
                                   int64_t groups, int64_t d_in, int64_t d_out, int activation,
                                   int dtype, void* workspace, hipStream_t stream) {
   PULSAR_REQUIRE(offsets, "grouped_linear_forward: null pointer");
-  return forward(Call{x, x_rs, x_rows, row_index, offsets, Weight{w, w_group, w_in, w_out}, rows,
+  return forward(Call{x, x_rs, x_rows, row_index, offsets, true, Weight{w, w_group, w_in, w_out}, rows,
                       groups, d_in, d_out, activation, dtype, "grouped_linear_forward"},
                  bias, bias_dtype, nullptr, 0, y, pre, workspace, stream);
 }
@@ -792,7 +870,7 @@ int64_t pulsar_grouped_linear_backward_workspace_bytes(const void* dy, const voi
                                                        int64_t w_group, int64_t w_in, int64_t w_out,
                                                        int64_t rows, int64_t groups, int64_t d_in,
                                                        int64_t d_out, int activation, int dtype) {
-  return backward_bytes(Call{x, x_rs, x_rows, nullptr, nullptr, Weight{w, w_group, w_in, w_out}, rows,
+  return backward_bytes(Call{x, x_rs, x_rows, nullptr, nullptr, true, Weight{w, w_group, w_in, w_out}, rows,
                              groups, d_in, d_out, activation, dtype, "grouped_linear_backward"}, dy);
 }
 
@@ -803,7 +881,7 @@ int pulsar_grouped_linear_backward(const void* dy, const void* x, int64_t x_rs, 
                                    int64_t d_in, int64_t d_out, int activation, int dtype,
                                    void* workspace, hipStream_t stream) {
   PULSAR_REQUIRE(offsets, "grouped_linear_backward: null pointer");
-  return backward(Call{x, x_rs, x_rows, row_index, offsets, Weight{w, w_group, w_in, w_out}, rows,
+  return backward(Call{x, x_rs, x_rows, row_index, offsets, true, Weight{w, w_group, w_in, w_out}, rows,
                        groups, d_in, d_out, activation, dtype, "grouped_linear_backward"},
                   dy, pre, dx, dw, db, workspace, stream);
 }

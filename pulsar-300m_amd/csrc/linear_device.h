@@ -754,10 +754,19 @@ __device__ __forceinline__ void finish_values(const LinearArgs& a, int act, int6
     for (int q = 0; q < 8; ++q) v[q] += x[q];
   }
 }
-// The same, stored with one rounding.
-template <typename T, bool PAIR>
+// 8 partial sums of row r from column col on, of split blockIdx.y.
+__device__ __forceinline__ void store_part(const LinearArgs& a, int64_t r, int col, int f, const float (&v)[8]) {
+  store_run<8>(a.part + ((int64_t)blockIdx.y * a.rows + r) * a.N + col, v, f - col);
+}
+// The same, stored with one rounding, or the sums of one of the splits (SPLIT).
+template <typename T, bool PAIR, bool SPLIT>
 __device__ __forceinline__ void finish_run(const LinearArgs& a, int act, int64_t r, int col, int f,
                                            float (&v)[8], float (&u)[8], const float (&bias)[2][8]) {
+  if (SPLIT && a.part) {
+    store_part(a, r, col, f, v);
+    if constexpr (PAIR) store_part(a, r, f + col, 2 * f, u);
+    return;
+  }
   float pre[8];
   finish_values<T, PAIR>(a, act, r, col, f, v, u, pre, bias);
   const int n = f - col;
@@ -838,13 +847,25 @@ struct EpilogueBias {
 // Epilogue of a product's tile. The wave's accumulators start at row r0 and output column c0; of
 // `f` output columns and rows below r1 only those inside are stored. PAIR: the second half of the
 // CT tiles are the up-projection twins of the first.
-template <typename T, Map MAP, int BW, bool PAIR, int RT>
+template <typename T, Map MAP, int BW, bool PAIR, bool SPLIT, int RT>
 __device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&acc)[RT][Slab::CT],
                                               Slab slab, const EpilogueBias<T, MAP, PAIR>& bias,
                                               bool none, int r0, int r1, int c0, int f) {
   constexpr int NCT = PAIR ? Slab::CT / 2 : Slab::CT;
   const int lane = (int)threadIdx.x & 63, act = none ? PULSAR_ACT_NONE : a.act;
   if constexpr (sizeof(T) == 2 && !PAIR) {
+    if (SPLIT && a.part) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          float v[8];
+          take_run<MAP>(acc[i][2 * p], acc[i][2 * p + 1], v);
+          const int r = r0 + 16 * i + (lane & 15), col = c0 + 32 * p + run_col<MAP>(lane >> 4);
+          if (r < r1 && col < f) store_part(a, r, col, f, v);
+        }
+      return;
+    }
     const PairStore<MAP> out(reinterpret_cast<bf16*>(a.C), a.ldc, 16 * RT, r0, r1, c0, f);
     if (act == PULSAR_ACT_NONE && !a.bias && !a.residual && !a.pre) {
 #pragma unroll
@@ -884,7 +905,7 @@ __device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&a
       take_run<MAP>(acc[i][0], acc[i][1], v);
       take_run<MAP>(acc[i][2], acc[i][3], u);
       const int64_t r = r0 + 16 * i + (lane & 15);
-      if (r < r1 && col < f) finish_run<T, PAIR>(a, act, r, col, f, v, u, bias.b[0]);
+      if (r < r1 && col < f) finish_run<T, PAIR, SPLIT>(a, act, r, col, f, v, u, bias.b[0]);
     }
     return;
   }
@@ -901,7 +922,7 @@ __device__ __forceinline__ void rows_epilogue(const LinearArgs& a, lin_f32x4 (&a
       float v[8], u[8] = {};
       slab.read8(p, 2 * lc, v);
       if constexpr (PAIR) slab.read8(p, 4 * NCT + 2 * lc, u);
-      finish_run<T, PAIR>(a, act, r, col, f, v, u, bias.slab);
+      finish_run<T, PAIR, SPLIT>(a, act, r, col, f, v, u, bias.slab);
     }
     lds_settle();  // read before the next rows overwrite
   }

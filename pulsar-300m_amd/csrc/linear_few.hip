@@ -71,12 +71,13 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
   const int lane = (int)threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int i16 = lane & 15, kq = lane >> 4;
 
-  // this wave's steps
-  const int all = none ? 0 : (a.K + KS - 1) / KS, per = (all + W - 1) / W;
+  // this workgroup's k's, and this wave's steps of them
+  int kfirst = 0, kend = a.K;
+  if (a.part) split_range<T>(a.K, a.splits, (int)blockIdx.y, kfirst, kend);
+  const int all = none ? 0 : (kend + KS - 1) / KS, per = (all + W - 1) / W;
   const int s0 = min(wv * per, all), s1 = min(s0 + per, all);
-  const int kend = a.K;
 
-  const T* Bp = reinterpret_cast<const T*>(a.B) + (none ? 0 : group) * a.b_group;
+  const T* Bp = reinterpret_cast<const T*>(a.B) + (none ? 0 : group) * a.b_group + kfirst * (BKC ? 1 : a.ldb);
   // column of tile t: gate tiles, then their twins
   auto tile_col = [&](int t) { return PAIR && t >= NCT ? a.up + n0 + (t - NCT) * 16 : n0 + t * 16; };
   auto tile_lim = [&](int t) { return PAIR && t >= NCT ? a.up + f : f; };
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
       r = none ? 0 : a.a_rows[r];
       in = r >= 0 && r < a.a_nrows;
     }
-    xp[i] = in ? reinterpret_cast<const T*>(a.A) + r * a.lda + kq * EV : nullptr;
+    xp[i] = in ? reinterpret_cast<const T*>(a.A) + r * a.lda + kfirst + kq * EV : nullptr;
   }
   auto load_x = [&](int s, uint4 (&x)[RT]) {
     const int k0 = s * KS;
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
         if constexpr (PAIR) u[q] += l[OBN + q];
       }
     }
-    finish_run<T, PAIR>(a, act, r, col, f, v, u, bias);
+    finish_run<T, PAIR, true>(a, act, r, col, f, v, u, bias);
   }
 }
 
@@ -243,7 +244,7 @@ int launch_few_shape(LinearArgs& a, hipStream_t s) {
   if (tiles > (int64_t)1 << 30) return fail(PULSAR_ERR_INVALID, "linear: launch too large");
   a.max_tiles = (int)tiles_r;
   linear_few_kernel<T, BKC, PAIR, RT, CT, W, D>
-      <<<(unsigned)((tiles + kXcds - 1) / kXcds * kXcds), 64 * W, 0, s>>>(a);
+      <<<dim3((unsigned)((tiles + kXcds - 1) / kXcds * kXcds), a.part ? a.splits : 1), 64 * W, 0, s>>>(a);
   PULSAR_LAUNCH_CHECK();
   return PULSAR_OK;
 }

@@ -450,7 +450,7 @@ def moe_group_rows(topk_idx: torch.Tensor, num_experts: int):
 
 def fused_linear_forward(x: torch.Tensor, weight: torch.Tensor, bias=None,
                          activation: str = "none", residual=None, save_pre: bool = False):
-    """act(x @ weight.T + bias) + residual in one launch: x [..., d_in], weight [d_out, d_in]
+    """act(x @ weight.T + bias) + residual, the epilogue fused: x [..., d_in], weight [d_out, d_in]
     (torch.nn.Linear's; either of its dimensions may be the contiguous one).
 
     activation: none, relu, silu, gelu (erf), gelu_tanh, sigmoid or swiglu (d_out / 2 columns:

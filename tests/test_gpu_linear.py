@@ -618,3 +618,61 @@ def test_linear_fp32_small_values(pc, M, I):
         t = (I + 2) * U * (x.double().abs() @ w.double().abs().t()) + 6 * I * 2.0 ** -149
         t += 2.0 ** -134 * (x.double().abs().sum(1, keepdim=True) + w.double().abs().sum(1))
         check(y, want, U * (want.abs() + t) + t, f"2^{a} 2^{b}")
+
+
+def _forward_workspace(x, w):
+    from pulsar_cuda import _lib
+
+    return _lib.load().pulsar_fused_linear_forward_workspace_bytes(
+        x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), *x.shape, w.shape[0], 0,
+        _lib.PULSAR_BF16 if x.dtype == torch.bfloat16 else _lib.PULSAR_F32)
+
+
+@pytest.mark.parametrize("dtype,M,I,O", [
+    ("bf16", 250, 4096, 4088), ("bf16", 256, 4104, 4096), ("bf16", 16000, 4096, 104),
+    ("fp32", 1, 4096, 1024), ("fp32", 17, 4100, 516), ("fp32", 300, 4096, 1000), ("fp32", 2331, 2056, 1024)])
+@pytest.mark.parametrize("order", ["oi", "io"])
+def test_linear_split_products(pc, dtype, M, I, O, order):
+    """Sums over a long k shared by workgroups: forward, and dx where d_out is the long side."""
+    dt = DT[dtype]
+    x, dy = rand(M, I, seed=1, dt=dt), rand(M, O, seed=4, dt=dt)
+    w = rand(O, I, seed=2, dt=dt, scale=I ** -0.5)
+    if order == "io":
+        w = w.t().contiguous().t()
+    if order == "oi" and I % 8 == 0:
+        split = _forward_workspace(x, w) >= 2 * M * O * 4
+        assert split or M == 16000
+    b = rand(O, seed=3, dt=torch.float32)
+    for act in ("none", "gelu", "relu", "swiglu"):
+        res = rand(M, O // 2 if act == "swiglu" else O, seed=5, dt=dt)
+        y, pre = pc.fused_linear_forward(x, w, b, act, res, save_pre=True)
+        check_forward(y, pre, x, w.t(), b, act, dt, res, what=act)
+        again = pc.fused_linear_forward(x, w, b, act, res)
+        assert torch.equal(y, again)
+    y = pc.fused_linear_forward(x, w)
+    check_forward(y, None, x, w.t(), None, "none", dt)
+    # the same matrix the other way round: its d_out is long, and dx's sum over it is split
+    ww, g = w.t(), rand(M, I, seed=6, dt=dt)
+    dx, dw, db = pc.fused_linear_backward(g, dy, ww, bias=True)
+    check_backward(dx, dw.t(), db, g, dy, ww.t(), g, "none", dt)
+
+
+@pytest.mark.parametrize("M", [17, 300])
+def test_linear_fp32_infinities_in_splits(pc, M):
+    """An infinite or NaN operand in one split's part of the sum reaches its rows or columns, and only those."""
+    I, O = 4096, 520
+    x, w = rand(M, I, seed=1, dt=torch.float32), rand(O, I, seed=2, dt=torch.float32)
+    clean = pc.fused_linear_forward(x, w)
+    x[3, 4000] = math.inf
+    x[5, 7] = math.nan
+    w[11, 2000] = -math.inf
+    y = pc.fused_linear_forward(x, w)
+    want = x.double() @ w.double().t()
+    odd = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y[odd].nan_to_num(1, 2, 3), want[odd].float().nan_to_num(1, 2, 3))
+    rows = torch.ones(M, dtype=torch.bool, device="cuda")
+    rows[[3, 5]] = False
+    cols = torch.arange(O, device="cuda") != 11
+    t = (I + 2) * U * (x[rows].double().abs() @ w[cols].double().abs().t())
+    check(y[rows][:, cols], want[rows][:, cols], U * (want[rows][:, cols].abs() + t) + t, "finite")
+    assert torch.isfinite(clean).all()
