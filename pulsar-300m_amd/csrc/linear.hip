@@ -329,6 +329,7 @@ struct PackJob {
   int64_t rows, src_ld, src_group;  // rows of each group
   int64_t chunks;                   // in all
   int cols, halves, run;
+  const int32_t* offsets;           // weights of groups without rows are left out (nullptr: none are)
 };
 struct PackJobs {
   PackJob job[3];
@@ -342,9 +343,10 @@ __global__ void __launch_bounds__(256) linear_pack_kernel(PackJobs jobs) {
   if (k == 3) return;
   const PackJob& j = jobs.job[k];
   const int per = j.run / W;
-  const int64_t run = i / per, row = run / j.halves;
+  const int64_t run = i / per, row = run / j.halves, group = row / j.rows;
+  if (j.offsets && j.offsets[group + 1] <= j.offsets[group]) return;
   const int c = (int)(i % per) * W, n = j.cols - c;
-  const U* p = reinterpret_cast<const U*>(j.src) + row / j.rows * j.src_group + row % j.rows * j.src_ld +
+  const U* p = reinterpret_cast<const U*>(j.src) + group * j.src_group + row % j.rows * j.src_ld +
                run % j.halves * j.cols + c;
   U v[W];
   if (n >= W) {
@@ -570,6 +572,7 @@ struct Matrix {
   const void* p;
   int64_t ld, group, groups, rows, cols;
   int halves = 1;  // of the columns
+  const int32_t* offsets = nullptr;  // weights of a ragged call: its groups
 };
 
 // Workspace handed out in 256-byte steps; with base == nullptr it only counts.
@@ -586,7 +589,8 @@ struct Space {
 // The kernels read operands in whole 16-byte chunks; a matrix whose rows do not lie that way (odd
 // widths, slices of wider buffers) is copied first, into rows padded with zeros. The copy costs
 // its bytes twice; reading such rows in place ran at a third of the aligned rate (517 rows x
-// 1023 x 777: 25-31 us).
+// 1023 x 777: 25-31 us). Of a ragged call's weights only groups that have rows are copied (4 rows
+// of 64 experts of 1023 x 1021: 64 -> 33 us).
 struct Packing {
   PackJobs jobs = {};
   int n = 0;
@@ -599,7 +603,7 @@ struct Packing {
     const int64_t run = round_up(cols, ev);
     PackJob& j = jobs.job[n++];
     j.src = m.p; j.rows = m.rows; j.src_ld = m.ld; j.src_group = m.group;
-    j.cols = (int)cols; j.halves = m.halves; j.run = (int)run;
+    j.cols = (int)cols; j.halves = m.halves; j.run = (int)run; j.offsets = m.offsets;
     m.ld = run * m.halves;
     m.group = m.rows * m.ld;
     j.chunks = m.groups * m.group / ev;
@@ -639,8 +643,8 @@ struct Call {
   int es() const { return dtype == PULSAR_BF16 ? 2 : 4; }
   Matrix x_matrix() const { return {x, x_rs, 0, 1, x_rows, d_in}; }
   Matrix w_matrix(bool pair) const {
-    if (in_contiguous(w)) return {w.p, w.out, w.group, groups, d_out, d_in};
-    return {w.p, w.in, w.group, groups, d_in, d_out, pair ? 2 : 1};
+    if (in_contiguous(w)) return {w.p, w.out, w.group, groups, d_out, d_in, 1, offsets};
+    return {w.p, w.in, w.group, groups, d_in, d_out, pair ? 2 : 1, offsets};
   }
   int check() const {
     const int rc = check_common(rows, groups, d_in, d_out, w, act, dtype, what);

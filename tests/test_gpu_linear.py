@@ -676,3 +676,35 @@ def test_linear_fp32_infinities_in_splits(pc, M):
     t = (I + 2) * U * (x[rows].double().abs() @ w[cols].double().abs().t())
     check(y[rows][:, cols], want[rows][:, cols], U * (want[rows][:, cols].abs() + t) + t, "finite")
     assert torch.isfinite(clean).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+@pytest.mark.parametrize("order", ["io", "oi"])
+def test_grouped_odd_widths_of_few_experts(pc, order, act, dtype):
+    """Odd rows are copied into padded ones, of the groups that have rows only: most have none, and
+    the weights of those are NaN."""
+    dt = DT[dtype]
+    E, I, O, counts = 70, 37, 42, {0: 3, 5: 1, 64: 20, 69: 2}
+    off = torch.tensor([0] + [counts.get(e, 0) for e in range(E)]).cumsum(0).to(torch.int32).cuda()
+    M = int(off[-1]) + 4  # and rows of no group
+    w = torch.full((E, I, O), math.nan, dtype=dt, device="cuda")
+    for e in counts:
+        w[e] = rand(I, O, seed=e, dt=dt, scale=I ** -0.5)
+    if order == "oi":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    cols = O // 2 if act == "swiglu" else O
+    x, dy = rand(M, I, seed=101, dt=dt), rand(M, cols, seed=102, dt=dt)
+    y, pre = pc.grouped_linear_forward(x, w, off, activation=act, save_pre=True)
+    dx, dw, db = pc.grouped_linear_backward(dy, x, w, off, None, pre, act, True)
+    start = 0
+    for e in range(E):
+        n = counts.get(e, 0)
+        r = slice(start, start + n)
+        if n:
+            check_forward(y[r], pre[r], x[r], w[e], None, act, dt, what=f"group {e}")
+            check_backward(dx[r], dw[e], db[e], dy[r], x[r], w[e], pre[r], act, dt, what=f"group {e}")
+        else:
+            assert not dw[e].any() and not db[e].any()
+        start += n
+    assert not y[start:].any() and not pre[start:].any() and not dx[start:].any()
